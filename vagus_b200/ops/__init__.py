@@ -13,7 +13,10 @@ from .ce import fused_linear_ce  # noqa: F401
 from .gdn import conv_silu, gdn_mixer, gdr_chunk, gdr_decode  # noqa: F401
 from .kda import kda_mixer  # noqa: F401
 from .kda import kda_chunk  # noqa: F401
+from .kvcache import Int4KV, int4_append, int4_attention, int4_read  # noqa: F401
 from .linear import linear, linear_residual  # noqa: F401
 from .mobius import mobius_scan  # noqa: F401
 from .pointwise import (embedding, qk_norm_rope, rmsnorm, rmsnorm_gated, rmsnorm_pass, sigmoid_gate,  # noqa: F401
                         swiglu)
+from .rotary import rotary  # noqa: F401
+from .verify import verify_draft  # noqa: F401

@@ -33,6 +33,8 @@ def check_error() -> None:
     code = _C.error_word()
     if code:
         _C.reset_error()
+        if code == 5:
+            raise RuntimeError("vagus_b200 kernel: an index given on the device (a start, a length) lies outside its cache")
         raise RuntimeError(f"vagus_b200 kernel watchdog tripped (code {code}): a device wait ran out of time")
 
 

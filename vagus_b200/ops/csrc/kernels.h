@@ -194,6 +194,70 @@ int mobius_bwd(const float* A, const float* B, const float* C, const float* D, c
                const float* gO, float* gA, float* gB, float* gC, float* gD, float* gx0, int batch, int L, int R,
                cudaStream_t st);
 
+// rotary.cu: rotary positions of q (B, L, H, D) and k (B, L, Hk, D) in one launch
+// (see rotary.cu); the outputs are dense.  type: 0 fp32, 1 fp16, 2 bf16.
+struct RotaryArgs {
+  const void *q, *k;                            // k unused when Hk == 0
+  void *yq, *yk;
+  long long sq_b, sq_l, sq_h, sk_b, sk_l, sk_h; // element strides (unit inner)
+  const void* pos; int pos_i64; long long pos_sb, pos_sl;   // positions, or null: offset + l
+  long long offset;
+  const double* inv;                            // (R / 2): angle a step of position
+  long long B, L; int H, Hk, D, R, interleaved;
+  float scale, sign;                            // sign -1: the transposed rotation
+};
+int rotary(const RotaryArgs& a, int type, cudaStream_t st);
+
+// kv4.cu: a key / value cache held in 4 bits (format: see kv4.cu).  codes (B, Hk, cap, D / 2)
+// uint8, params (B, Hk, cap, D / 32, 2) bf16; cap is a multiple of 16.  A start or length
+// given on the device that leaves the cache records kErrBadArgument and touches nothing outside.
+struct Kv4AppendArgs {
+  const void *k, *v;                            // (B, Hk, L, D | Dv)
+  long long sk_b, sk_h, sk_l, sv_b, sv_h, sv_l;
+  void *k_codes, *k_params, *v_codes, *v_params;
+  const void* start; int start_i64; long long offset;       // per sequence, or null: offset
+  long long B, L, cap; int Hk, D, Dv;
+  int* err;
+};
+int kv4_append(const Kv4AppendArgs& a, int type, cudaStream_t st);
+struct Kv4ReadArgs {
+  const void *k_codes, *k_params, *v_codes, *v_params;
+  void *k, *v;                                  // (B, Hk, L, D | Dv) bf16 dense
+  const void* start; int start_i64; long long offset;
+  long long B, L, cap; int Hk, D, Dv;
+  int* err;
+};
+int kv4_read(const Kv4ReadArgs& a, cudaStream_t st);
+struct Kv4AttnArgs {
+  const void* q;                                // (B, H, Lq, D) bf16, strides multiples of 8 elements
+  long long sq_b, sq_h, sq_l;
+  const unsigned char *k_codes, *v_codes;
+  const void *k_params, *v_params;
+  void* o;                                      // (B, Lq, H, Dv) bf16 dense
+  const void* lengths; int len_i64; long long length;       // tokens held per sequence, or null: length
+  long long B, cap; int H, Hk, Lq, D, Dv, causal, splits;
+  float scale_log2;                             // softmax scale times log2(e)
+  float *part_o, *part_ml;                      // (B, Lq, H, splits, Dv | 2) fp32 when splits > 1
+  int* err;
+};
+int kv4_attn_tiles(const Kv4AttnArgs& a);
+int kv4_attn_splits(const Kv4AttnArgs& a, long long most_tokens);
+int kv4_attn(const Kv4AttnArgs& a, cudaStream_t st);
+
+// verify.cu: verification of drafted tokens (see verify.cu).  type: 0 fp32, 1 fp16, 2 bf16.
+struct VerifyArgs {
+  const void* target; long long st_b, st_k;     // (B, K + 1, V)
+  const void* draft; long long sd_b, sd_k;      // (B, K, V), or null: the drafts were certain
+  const long long* tokens; long long stok_b;    // (B, K)
+  const float* u_accept; long long su_b;        // (B, K)
+  const float* u_sample;                        // (B)
+  const void* lengths; int len_i64;             // drafted tokens per row, or null: K
+  long long* out;                               // (B, K + 1)
+  long long* accepted;                          // (B)
+  long long B, V; int K;
+};
+int verify_draft(const VerifyArgs& a, int type, cudaStream_t st);
+
 // comm.cu: NVLink peer-to-peer all-gather / reduce-scatter over CUDA-IPC
 // shared heaps (see comm.cu for the heap layout and the epoch protocol).
 constexpr int kMaxCommPeers = 16;

@@ -1,0 +1,195 @@
+// Rotary positions of queries and keys, one launch for both, forward and (with
+// the angles negated) backward:
+//
+//   y_a = m (x_a cos t - x_b sin t),  y_b = m (x_a sin t + x_b cos t),
+//   t = position * inv_freq[i],  i = 0 .. R / 2 - 1,
+//
+// over the channel pairs (a, b) = (2 i, 2 i + 1) (interleaved) or
+// (i, i + R / 2) (half); channels R .. D - 1 pass through.
+//
+// The angle of a far position needs more than 32 bits (a position of 2^20 times
+// a frequency of 1 leaves a float 0.06 rad of step), so it is formed in 64 bits
+// and reduced to a fraction of a turn before the 32-bit sine and cosine; the
+// products are 32-bit, rounded once to the output type.  A CTA takes a few
+// tokens: its threads first form the tokens' R / 2 angles, one each, in shared
+// memory, then stream every head of q and k past them with 16-byte accesses, so
+// an angle is computed once per token and not once per head.  What bounds it is
+// the HBM traffic of q and k, read once and written once.
+#include "common.cuh"
+#include "kernels.h"
+
+namespace vagus {
+namespace {
+
+template <typename T> __device__ __forceinline__ float to_f(T v);
+template <> __device__ __forceinline__ float to_f(float v) { return v; }
+template <> __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_f(float v);
+template <> __device__ __forceinline__ float from_f(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
+
+template <typename T>
+struct alignas(16) Vec {
+  static constexpr int N = 16 / sizeof(T);
+  T v[N];
+};
+
+constexpr int kThreads = 256;
+constexpr int kMaxAngles = 1024;     // pairs of angles of a CTA's tokens in shared memory
+
+__device__ __forceinline__ long long position_of(const RotaryArgs& a, long long b, long long l) {
+  if (a.pos == nullptr) return a.offset + l;
+  const long long i = b * a.pos_sb + l * a.pos_sl;
+  return a.pos_i64 ? static_cast<const long long*>(a.pos)[i] : static_cast<const int*>(a.pos)[i];
+}
+
+__device__ __forceinline__ float2 angle_of(double pos, double inv, float m, float sign) {
+  const double turns = pos * inv * 0.15915494309189533577;      // 1 / (2 pi)
+  const float f = static_cast<float>(turns - rint(turns));
+  float s, c;
+  sincospif(2.f * f, &s, &c);
+  return make_float2(c * m, s * m * sign);
+}
+
+// one row (token, head) of either tensor
+template <typename T>
+__device__ __forceinline__ void row_of(const RotaryArgs& a, long long b, long long l, int h, const T*& src, T*& dst) {
+  if (h < a.H) {
+    src = static_cast<const T*>(a.q) + b * a.sq_b + l * a.sq_l + h * a.sq_h;
+    dst = static_cast<T*>(a.yq) + ((b * a.L + l) * a.H + h) * a.D;
+  } else {
+    h -= a.H;
+    src = static_cast<const T*>(a.k) + b * a.sk_b + l * a.sk_l + h * a.sk_h;
+    dst = static_cast<T*>(a.yk) + ((b * a.L + l) * a.Hk + h) * a.D;
+  }
+}
+
+// blockDim = (items of a head, heads); an item is one 16-byte vector, or for the
+// half layout's rotated channels the two vectors that pair up.
+template <typename T, bool INTER>
+__global__ void __launch_bounds__(kThreads) rotary_vec_k(const RotaryArgs a, int tokens) {
+  constexpr int N = Vec<T>::N;
+  extern __shared__ float2 cs[];                                  // [tokens][R / 2]
+  const int half = a.R / 2, tid = threadIdx.y * blockDim.x + threadIdx.x, nthr = blockDim.x * blockDim.y;
+  const long long t0 = static_cast<long long>(blockIdx.x) * tokens, total = a.B * a.L;
+  const int nt = static_cast<int>(min(static_cast<long long>(tokens), total - t0));
+  for (int i = tid; i < nt * half; i += nthr) {
+    const int tk = i / half, p = i - tk * half;
+    const long long t = t0 + tk, b = t / a.L, l = t - b * a.L;
+    cs[i] = angle_of(static_cast<double>(position_of(a, b, l)), a.inv[p], a.scale, a.sign);
+  }
+  __syncthreads();
+  const int heads = a.H + a.Hk, item = threadIdx.x;
+  const int rot = INTER ? a.R / N : half / N;                     // items that rotate
+  for (int tk = 0; tk < nt; ++tk) {
+    const long long t = t0 + tk, b = t / a.L, l = t - b * a.L;
+    const float2* c = cs + tk * half;
+    for (int h = threadIdx.y; h < heads; h += blockDim.y) {
+      const T* src;
+      T* dst;
+      row_of<T>(a, b, l, h, src, dst);
+      if (INTER) {
+        const int c0 = item * N;
+        Vec<T> x = *reinterpret_cast<const Vec<T>*>(src + c0);
+        if (item < rot) {
+#pragma unroll
+          for (int j = 0; j < N; j += 2) {
+            const float2 w = c[(c0 + j) / 2];
+            const float xa = to_f(x.v[j]), xb = to_f(x.v[j + 1]);
+            x.v[j] = from_f<T>(xa * w.x - xb * w.y);
+            x.v[j + 1] = from_f<T>(xa * w.y + xb * w.x);
+          }
+        }
+        *reinterpret_cast<Vec<T>*>(dst + c0) = x;
+      } else if (item < rot) {
+        const int c0 = item * N;
+        Vec<T> xa = *reinterpret_cast<const Vec<T>*>(src + c0);
+        Vec<T> xb = *reinterpret_cast<const Vec<T>*>(src + half + c0);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const float2 w = c[c0 + j];
+          const float fa = to_f(xa.v[j]), fb = to_f(xb.v[j]);
+          xa.v[j] = from_f<T>(fa * w.x - fb * w.y);
+          xb.v[j] = from_f<T>(fa * w.y + fb * w.x);
+        }
+        *reinterpret_cast<Vec<T>*>(dst + c0) = xa;
+        *reinterpret_cast<Vec<T>*>(dst + half + c0) = xb;
+      } else {
+        const int c0 = a.R + (item - rot) * N;
+        *reinterpret_cast<Vec<T>*>(dst + c0) = *reinterpret_cast<const Vec<T>*>(src + c0);
+      }
+    }
+  }
+}
+
+// any D, even R, any alignment: one channel pair (or one passed channel) a thread
+template <typename T>
+__global__ void __launch_bounds__(kThreads) rotary_any_k(const RotaryArgs a, int tokens) {
+  extern __shared__ float2 cs[];
+  const int half = a.R / 2;
+  const long long t0 = static_cast<long long>(blockIdx.x) * tokens, total = a.B * a.L;
+  const int nt = static_cast<int>(min(static_cast<long long>(tokens), total - t0));
+  for (int i = threadIdx.x; i < nt * half; i += blockDim.x) {
+    const int tk = i / half, p = i - tk * half;
+    const long long t = t0 + tk, b = t / a.L, l = t - b * a.L;
+    cs[i] = angle_of(static_cast<double>(position_of(a, b, l)), a.inv[p], a.scale, a.sign);
+  }
+  __syncthreads();
+  const int items = half + a.D - a.R, heads = a.H + a.Hk;
+  for (int i = threadIdx.x; i < nt * heads * items; i += blockDim.x) {
+    const int r = i / items, it = i - r * items, tk = r / heads;
+    const long long t = t0 + tk, b = t / a.L, l = t - b * a.L;
+    const T* src;
+    T* dst;
+    row_of<T>(a, b, l, r - tk * heads, src, dst);
+    if (it < half) {
+      const int ca = a.interleaved ? 2 * it : it, cb = a.interleaved ? 2 * it + 1 : it + half;
+      const float2 w = cs[tk * half + it];
+      const float xa = to_f(src[ca]), xb = to_f(src[cb]);
+      dst[ca] = from_f<T>(xa * w.x - xb * w.y);
+      dst[cb] = from_f<T>(xa * w.y + xb * w.x);
+    } else {
+      dst[it + half] = src[it + half];
+    }
+  }
+}
+
+template <typename T>
+int launch(const RotaryArgs& a, cudaStream_t st) {
+  constexpr int N = Vec<T>::N;
+  const int half = a.R / 2;
+  // tokens a CTA: as many as its threads have angles for at once, fewer while the grid would not fill the GPU
+  int tokens = half >= kThreads ? 1 : kThreads / half;
+  while (tokens > 1 && (a.B * a.L + tokens - 1) / tokens < 148 * 4) --tokens;
+  const long long grid = (a.B * a.L + tokens - 1) / tokens;
+  if (grid > 0x7fffffffLL) return 2;
+  const size_t smem = static_cast<size_t>(tokens) * half * sizeof(float2);
+  auto al = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+  auto mul = [](long long s) { return s % N == 0; };
+  const bool vec = al(a.q) && al(a.yq) && mul(a.sq_b) && mul(a.sq_l) && mul(a.sq_h) &&
+                   (a.Hk == 0 || (al(a.k) && al(a.yk) && mul(a.sk_b) && mul(a.sk_l) && mul(a.sk_h))) &&
+                   a.D % N == 0 && (a.interleaved ? a.R % N == 0 : half % N == 0);
+  const int items = vec ? (a.interleaved ? a.D / N : half / N + (a.D - a.R) / N) : 0;
+  if (vec && items <= kThreads) {
+    const dim3 block(items, kThreads / items);
+    if (a.interleaved) rotary_vec_k<T, true><<<static_cast<unsigned>(grid), block, smem, st>>>(a, tokens);
+    else rotary_vec_k<T, false><<<static_cast<unsigned>(grid), block, smem, st>>>(a, tokens);
+  } else {
+    rotary_any_k<T><<<static_cast<unsigned>(grid), kThreads, smem, st>>>(a, tokens);
+  }
+  return cudaGetLastError() == cudaSuccess ? 0 : 3;
+}
+
+}  // namespace
+
+int rotary(const RotaryArgs& a, int type, cudaStream_t st) {
+  if (a.R < 2 || a.R % 2 || a.R > a.D || a.R / 2 > kMaxAngles) return 1;
+  if (a.B * a.L == 0 || a.H + a.Hk == 0) return 0;
+  if (type == 0) return launch<float>(a, st);
+  if (type == 1) return launch<__half>(a, st);
+  return launch<__nv_bfloat16>(a, st);
+}
+
+}  // namespace vagus

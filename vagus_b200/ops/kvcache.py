@@ -1,0 +1,234 @@
+"""A key / value cache held in 4 bits, and softmax attention over it.
+
+For every (sequence, KV head, token) the cache holds one 4-bit code a channel
+(channel 2 j in the low half of byte j) and, for each group of 32 channels, a
+step s and an offset b in bf16:
+
+    s = bf16((max - min) / 15),  b = bf16(min - 128 s),
+    c = clamp(round((x - b) / s) - 128, 0, 15),  and c stands for bf16((128 + c) s + b)
+
+(round: to nearest, ties to even; the steps in fp32).  That is 0.625 bytes a
+value against 2 of a bf16 cache, and a value is off by little more than half a
+step.  A group of equal values is held exactly (s = 0); a group that holds a NaN
+or an infinity stands for NaN; magnitudes up to 1e37 are representable.
+
+``int4_attention`` is attention over the values that the codes stand for, which
+``int4_read`` returns: however a stream is cut into calls, a token sees the same
+keys and values.  CUDA runs ``kv4.cu``; elsewhere the plain forms below run.
+"""
+
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+
+import torch
+
+from ._core import native
+
+GROUP = 32
+_BLOCK = 16         # the capacity is a whole number of blocks of this many tokens
+
+
+@dataclass
+class Int4KV:
+    """The four tensors of a cache, all contiguous on one device: codes
+    (B, Hk, capacity, D / 2) uint8 and parameters (B, Hk, capacity, D / 32, 2)
+    bf16 holding (s, b), for keys and for values."""
+    k_codes: torch.Tensor
+    k_params: torch.Tensor
+    v_codes: torch.Tensor
+    v_params: torch.Tensor
+
+    def __post_init__(self):
+        for codes, params, what in ((self.k_codes, self.k_params, "k"), (self.v_codes, self.v_params, "v")):
+            if codes.dim() != 4 or codes.dtype != torch.uint8 or not codes.is_contiguous() \
+                    or codes.shape[3] % (GROUP // 2) or not codes.shape[3]:
+                raise ValueError(f"Int4KV: {what}_codes must be (B, Hk, capacity, D / 2) uint8, contiguous, "
+                                 f"D a multiple of {GROUP}")
+            want = (*codes.shape[:3], codes.shape[3] * 2 // GROUP, 2)
+            if tuple(params.shape) != want or params.dtype != torch.bfloat16 or not params.is_contiguous():
+                raise ValueError(f"Int4KV: {what}_params must be {want} bf16, contiguous")
+        if self.k_codes.shape[:3] != self.v_codes.shape[:3]:
+            raise ValueError("Int4KV: keys and values must agree in batch, heads and capacity")
+        if self.capacity % _BLOCK:
+            raise ValueError(f"Int4KV: the capacity must be a multiple of {_BLOCK}")
+        if any(t.device != self.k_codes.device for t in self.tensors()):
+            raise ValueError("Int4KV: the tensors must be on one device")
+
+    @classmethod
+    def empty(cls, batch: int, kv_heads: int, capacity: int, head_dim: int, value_dim: int | None = None,
+              device=None) -> "Int4KV":
+        """Room for at least ``capacity`` tokens of ``batch`` sequences, zeroed."""
+        value_dim = head_dim if value_dim is None else value_dim
+        if head_dim < GROUP or head_dim % GROUP or value_dim < GROUP or value_dim % GROUP:
+            raise ValueError(f"Int4KV: head dims must be multiples of {GROUP}, got {head_dim} and {value_dim}")
+        cap = -(-capacity // _BLOCK) * _BLOCK
+
+        def pair(d):
+            return (torch.zeros(batch, kv_heads, cap, d // 2, dtype=torch.uint8, device=device),
+                    torch.zeros(batch, kv_heads, cap, d // GROUP, 2, dtype=torch.bfloat16, device=device))
+        return cls(*pair(head_dim), *pair(value_dim))
+
+    def tensors(self) -> tuple[torch.Tensor, ...]:
+        return self.k_codes, self.k_params, self.v_codes, self.v_params
+
+    @property
+    def batch(self) -> int:
+        return self.k_codes.shape[0]
+
+    @property
+    def kv_heads(self) -> int:
+        return self.k_codes.shape[1]
+
+    @property
+    def capacity(self) -> int:
+        return self.k_codes.shape[2]
+
+    @property
+    def head_dim(self) -> int:
+        return 2 * self.k_codes.shape[3]
+
+    @property
+    def value_dim(self) -> int:
+        return 2 * self.v_codes.shape[3]
+
+
+# ------------------------------------------------------------------ plain forms --
+
+def int4_quantise_ref(x):
+    """(..., D) -> codes (..., D / 2) uint8 and parameters (..., D / 32, 2) bf16."""
+    g = x.float().unflatten(-1, (-1, GROUP))
+    lo, hi = g.amin(-1, keepdim=True), g.amax(-1, keepdim=True)
+    s = ((hi - lo) / 15).bfloat16().float()
+    b = (lo - 128 * s).bfloat16().float()
+    c = (torch.round((g - b) / s) - 128).clamp(0, 15)
+    c = torch.where((s > 0) & ~c.isnan(), c, torch.zeros_like(c)).flatten(-2).to(torch.uint8)
+    return c[..., 0::2] | (c[..., 1::2] << 4), torch.cat((s, b), -1).bfloat16()
+
+
+def int4_values_ref(codes, params):
+    """The bf16 values that codes stand for."""
+    c = torch.stack((codes & 15, codes >> 4), -1).flatten(-2).float().unflatten(-1, (-1, GROUP))
+    return ((c + 128) * params[..., :1].float() + params[..., 1:].float()).flatten(-2).bfloat16()
+
+
+def int4_attention_ref(q, k, v, lengths, causal: bool = True):
+    """q (B, H, Lq, D) over k, v (B, Hk, T, ..), of which sequence b holds ``lengths[b]`` tokens."""
+    B, H, Lq, D = q.shape
+    Hk, T = k.shape[1], k.shape[2]
+    up = torch.promote_types(q.dtype, torch.float32)
+    at = torch.arange(T, device=q.device)
+    held = at < lengths[:, None]
+    # what lies past a sequence's length counts nothing, whatever it is
+    k = torch.where(held[:, None, :, None], k, 0.0).to(up)
+    v = torch.where(held[:, None, :, None], v, 0.0).to(up)
+    s = q.to(up).reshape(B, Hk, H // Hk * Lq, D) @ k.transpose(-1, -2) / math.sqrt(D)
+    s = s.view(B, Hk, H // Hk, Lq, T)
+    seen = lengths[:, None] - Lq + 1 + torch.arange(Lq, device=q.device) if causal else lengths[:, None].expand(B, Lq)
+    s = s.masked_fill(at >= seen[:, None, None, :, None], float("-inf"))
+    top = s.amax(-1, keepdim=True) if T else s.new_zeros(B, Hk, H // Hk, Lq, 1)
+    p = torch.exp(s - torch.where(top == float("-inf"), torch.zeros_like(top), top))
+    total = p.sum(-1, keepdim=True)
+    p = p / torch.where(total == 0, torch.ones_like(total), total)     # a row that sees nothing gives zeros
+    return (p.view(B, Hk, H // Hk * Lq, T) @ v).view(B, H, Lq, -1).to(q.dtype)
+
+
+# ------------------------------------------------------------------ entry points --
+
+def _per_row(x, cache: Int4KV, what: str):
+    """(tensor or None, int) of a place given as an int or per sequence."""
+    if isinstance(x, torch.Tensor):
+        if x.dtype not in (torch.int32, torch.int64) or tuple(x.shape) != (cache.batch,) \
+                or x.device != cache.k_codes.device:
+            raise ValueError(f"{what} must be an int or ({cache.batch},) int32 / int64 on the cache's device")
+        return x.contiguous(), 0
+    if not isinstance(x, int):
+        raise ValueError(f"{what} must be an int or a tensor")
+    return None, x
+
+
+def _rows(per, at, cache):
+    return per.to(torch.int64) if per is not None else torch.full((cache.batch,), at, device=cache.k_codes.device)
+
+
+def _span(cache: Int4KV, per, at: int, count: int, what: str):
+    """Host-side check of tokens [start, start + count)."""
+    if per is None:
+        ok = 0 <= at and at + count <= cache.capacity
+    else:
+        # a start on the GPU is checked there (``check_error`` reports it)
+        ok = per.is_cuda or per.numel() == 0 or (int(per.min()) >= 0 and int(per.max()) + count <= cache.capacity)
+    if count < 0 or not ok:
+        raise ValueError(f"{what}: tokens outside the cache of {cache.capacity}")
+
+
+@torch.no_grad()
+def int4_append(cache: Int4KV, k, v, start) -> None:
+    """Quantise ``k`` (B, Hk, L, D) and ``v`` (B, Hk, L, Dv) into the cache as
+    tokens start .. start + L - 1 (``start``: an int, or (B,) int32 / int64 for
+    a place per sequence; one given on the GPU is checked by the kernel, which
+    writes nothing outside the cache and reports it through ``check_error``)."""
+    if k.dim() != 4 or v.dim() != 4 or k.shape[:3] != v.shape[:3] or k.shape[0] != cache.batch \
+            or k.shape[1] != cache.kv_heads or k.shape[3] != cache.head_dim or v.shape[3] != cache.value_dim:
+        raise ValueError(f"int4_append: k {tuple(k.shape)}, v {tuple(v.shape)} do not fit the cache")
+    if k.dtype != v.dtype or k.device != cache.k_codes.device or v.device != cache.k_codes.device:
+        raise ValueError("int4_append: k and v must share a dtype and be on the cache's device")
+    per, at = _per_row(start, cache, "int4_append: start")
+    L = k.shape[2]
+    _span(cache, per, at, L, "int4_append")
+    if k.is_cuda:
+        if k.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+            raise ValueError(f"int4_append: {k.dtype} on the GPU (fp32, fp16 or bf16)")
+        k, v = (x if x.stride(-1) == 1 else x.contiguous() for x in (k, v))
+        native().kv4_append(*cache.tensors(), k, v, per, at)
+        return
+    i = torch.arange(cache.batch)[:, None, None]
+    j = torch.arange(cache.kv_heads)[None, :, None]
+    t = _rows(per, at, cache)[:, None, None] + torch.arange(L)
+    for have, new in zip(cache.tensors(), int4_quantise_ref(k) + int4_quantise_ref(v)):
+        have[i, j, t] = new
+
+
+@torch.no_grad()
+def int4_read(cache: Int4KV, start, count: int):
+    """The values of tokens start .. start + count - 1 as bf16 k (B, Hk, count, D)
+    and v (B, Hk, count, Dv); ``start`` as in ``int4_append`` (tokens outside
+    the cache read as zeros on the GPU and are reported)."""
+    per, at = _per_row(start, cache, "int4_read: start")
+    _span(cache, per, at, count, "int4_read")
+    if cache.k_codes.is_cuda:
+        return tuple(native().kv4_read(*cache.tensors(), per, at, count))
+    i = torch.arange(cache.batch)[:, None, None]
+    j = torch.arange(cache.kv_heads)[None, :, None]
+    t = _rows(per, at, cache)[:, None, None] + torch.arange(count)
+    kc, kp, vc, vp = (x[i, j, t] for x in cache.tensors())
+    return int4_values_ref(kc, kp), int4_values_ref(vc, vp)
+
+
+@torch.no_grad()
+def int4_attention(q, cache: Int4KV, lengths, causal: bool = True):
+    """Attention of ``q`` (B, H, Lq, D) over the first ``lengths`` tokens of the
+    cache -> (B, H, Lq, Dv); H is a multiple of the cache's heads.
+
+    ``lengths``: an int, or (B,) int32 / int64 (given on the GPU, the kernel
+    clamps it to the cache and reports it through ``check_error``).  With
+    ``causal`` the queries are the last Lq of those tokens: query i sees the
+    first lengths - Lq + i + 1 of them.  A query that sees nothing gives zeros.
+    What the cache holds past a sequence's length has no effect.  Inference
+    only: no gradient flows."""
+    if q.dim() != 4 or q.shape[0] != cache.batch or q.shape[3] != cache.head_dim or not cache.kv_heads \
+            or q.shape[1] % cache.kv_heads:
+        raise ValueError(f"int4_attention: q {tuple(q.shape)} does not fit the cache")
+    if q.device != cache.k_codes.device:
+        raise ValueError("int4_attention: q must be on the cache's device")
+    per, at = _per_row(lengths, cache, "int4_attention: lengths")
+    if per is None:
+        if not 0 <= at <= cache.capacity:
+            raise ValueError(f"int4_attention: {at} tokens in a cache of {cache.capacity}")
+    elif not per.is_cuda and per.numel() and int(per.max()) > cache.capacity:
+        raise ValueError(f"int4_attention: lengths exceed the cache of {cache.capacity}")
+    if q.is_cuda and q.dtype == torch.bfloat16 and cache.head_dim in (64, 128) and cache.value_dim in (64, 128):
+        return native().kv4_attn(q, *cache.tensors(), per, at, bool(causal), 1.0 / math.sqrt(q.shape[-1]))
+    k, v = int4_read(cache, 0, cache.capacity if per is not None else at)
+    return int4_attention_ref(q, k, v, _rows(per, at, cache).clamp(0, cache.capacity), causal)
