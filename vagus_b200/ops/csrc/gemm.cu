@@ -676,6 +676,14 @@ EncodeFn get_encode() {
       std::fprintf(stderr, "[gemm] entry point rc %d status %d ptr %p\n", (int)e, (int)q, ptr);
     if (e == cudaSuccess && q == cudaDriverEntryPointSuccess) fn = reinterpret_cast<EncodeFn>(ptr);
   });
+  // The encoder is a driver call: it wants a context current on the calling
+  // thread, which a thread whose first CUDA work this is (an autograd worker
+  // served from cached memory, say) does not have until a runtime call binds it.
+  static thread_local bool bound = false;
+  if (!bound) {
+    int dev = 0;
+    bound = cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess;
+  }
   return fn;
 }
 
