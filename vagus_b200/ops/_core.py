@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import weakref
+
 import torch
 
 _C = None
@@ -40,10 +42,12 @@ def check_error() -> None:
 
 class _Bf16Cache:
     """bf16 compute copies of fp32 master weights, rebuilt when the master
-    changes (its autograd version counter moves on every in-place update)."""
+    changes (its autograd version counter moves on every in-place update).  An
+    entry holds a weak reference to its master: a new tensor that takes a dead
+    one's id and memory is another master."""
 
     def __init__(self):
-        self._d: dict[int, tuple[int, int, torch.Tensor]] = {}
+        self._d: dict = {}
 
     def get(self, w: torch.Tensor) -> torch.Tensor:
         if w.dtype == torch.bfloat16:
@@ -51,10 +55,10 @@ class _Bf16Cache:
         key = id(w)
         ver = w._version
         hit = self._d.get(key)
-        if hit is not None and hit[0] == ver and hit[1] == w.data_ptr():
+        if hit is not None and hit[0] == ver and hit[1] == w.data_ptr() and hit[3]() is w:
             return hit[2]
         c = w.detach().to(torch.bfloat16).contiguous()
-        self._d[key] = (ver, w.data_ptr(), c)
+        self._d[key] = (ver, w.data_ptr(), c, weakref.ref(w))
         return c
 
     def get_cat(self, ws: list[torch.Tensor]) -> torch.Tensor:
@@ -66,10 +70,10 @@ class _Bf16Cache:
         key = ("cat",) + tuple(id(w) for w in ws)
         vers = tuple((w._version, w.data_ptr()) for w in ws)
         hit = self._d.get(key)
-        if hit is not None and hit[0] == vers:
+        if hit is not None and hit[0] == vers and all(r() is w for r, w in zip(hit[3], ws)):
             return hit[2]
         c = torch.cat([w.detach().to(torch.bfloat16) for w in ws], 0).contiguous()
-        self._d[key] = (vers, None, c)
+        self._d[key] = (vers, None, c, [weakref.ref(w) for w in ws])
         return c
 
     def clear(self):
