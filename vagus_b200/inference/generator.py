@@ -21,6 +21,11 @@ when every row has produced a stop id; the stop test is the only per-token
 read of device data, and it is skipped when there are no stop ids, so a
 run without stop ids queues all its decode steps without waiting on the GPU.
 
+``gen_ids_drafted`` generates with a second, smaller generator that drafts
+several tokens ahead: one model call checks them all (``ops.verify_draft``), and
+what comes out is distributed as this generator's own samples.  ``cache_bits=4``
+holds the softmax layers' KV caches in 4 bits.
+
 Batches are (B, L) with equal-length rows (the decode step takes no padding
 mask).  ``score_ids`` is teacher-forced scoring through the same decode path
 (fresh streams, one feed with logits), so evaluation needs nothing of a model
@@ -38,9 +43,10 @@ from typing import Iterator, Sequence
 
 import torch
 
+from .. import ops
 from ..models.decodable import Decodable, missing_decodable
 from ..utils import infer_device
-from .sampling import SamplingConfig, sample
+from .sampling import SamplingConfig, probabilities, sample
 
 
 @dataclass
@@ -60,13 +66,19 @@ class Generator:
     (``tokenizers.Tokenizer``) for the text conveniences.  ``start_id`` is
     how a document starts (the head of a fresh stream), ``stop_ids`` how it
     ends (the default of ``SamplingConfig.stop_ids=None``); both belong to
-    the tokenizer's stream conventions, not to the model."""
+    the tokenizer's stream conventions, not to the model.  ``cache_bits``
+    (16 or 4; None leaves the model's setting) is the width of the softmax
+    layers' KV caches."""
 
     def __init__(self, model: Decodable, tokenizer=None, start_id: int | None = None,
-                 stop_ids: tuple[int, ...] = ()):
+                 stop_ids: tuple[int, ...] = (), cache_bits: int | None = None):
         missing = missing_decodable(model)
         if missing:
             raise TypeError(f"{type(model).__name__} does not implement Decodable: missing {missing}")
+        if cache_bits is not None:
+            if not hasattr(model, "set_cache_bits"):
+                raise TypeError(f"{type(model).__name__} has no cache_bits setting")
+            model.set_cache_bits(cache_bits)
         self.model = model
         self.tokenizer = tokenizer
         self.start_id = start_id
@@ -79,7 +91,7 @@ class Generator:
 
     @classmethod
     def from_checkpoint(cls, path, device="cpu", dtype=None, tokenizer_id: str | None = None,
-                        with_meta: bool = False):
+                        with_meta: bool = False, cache_bits: int | None = None):
         """Model, tokenizer and stream conventions from one checkpoint
         (``tokenizer_id`` overrides the checkpoint's record and is required
         when it has none).  ``with_meta`` also returns ``load_model``'s
@@ -91,7 +103,7 @@ class Generator:
         if tid is None:
             raise ValueError(f"{path} records no tokenizer; pass tokenizer_id=")
         start_id, stop_ids = tokenizers.stream_conventions(tid)
-        gen = cls(model, tokenizers.load(tid), start_id=start_id, stop_ids=stop_ids)
+        gen = cls(model, tokenizers.load(tid), start_id=start_id, stop_ids=stop_ids, cache_bits=cache_bits)
         return (gen, meta) if with_meta else gen
 
     # ------------------------------------------------------------ bookkeeping --
@@ -234,6 +246,91 @@ class Generator:
         if not toks:
             return torch.empty(self.streams.rows, 0, dtype=torch.int64, device=self.device)
         return torch.stack(toks, dim=1)
+
+    def _rewind(self, tokens: int) -> None:
+        if tokens:
+            self.model.rewind_cache(tokens)
+            self.streams.consumed -= tokens
+
+    @torch.no_grad()
+    def gen_ids_drafted(self, cfg: SamplingConfig, draft: "Generator", n_draft: int = 4) -> torch.Tensor:
+        """(B, N) int64 like ``gen_ids``, with ``draft``'s model guessing up to
+        ``n_draft`` tokens ahead of each call of this one.  ``draft`` must hold
+        the same streams (the same prompt prefilled) over the same vocabulary,
+        and both models must be able to drop their newest tokens
+        (``can_rewind``).  Every token is distributed as this generator's own
+        sample; at temperature 0 the tokens are the greedy ones.  The rows of a
+        batch advance together, by the shortest accepted run plus one.  Afterwards
+        both generators hold the streams with the generated tokens."""
+        s, d = self.streams, draft.streams
+        if n_draft < 1:
+            raise ValueError("n_draft must be at least 1")
+        if draft is self or draft.model is self.model:
+            raise ValueError("the draft must be another generator over another model")
+        for g in (self, draft):
+            if not getattr(g.model, "can_rewind", lambda: False)():
+                raise TypeError(f"drafted generation needs models whose streams can be rewound; "
+                                f"{type(g.model).__name__}'s cannot")
+        # before anything is fed: a drafted id beyond the target's embedding must not reach it
+        sizes = [getattr(g.model, "config", {}).get("vocab_size") for g in (self, draft)]
+        if None in sizes or sizes[0] != sizes[1]:
+            raise ValueError(f"the models must state one vocab_size in their config, got {sizes[0]} and {sizes[1]}")
+        if s.head is None or d.head is None:
+            raise RuntimeError("the streams are empty: prefill a prompt first (this tokenizer has no start token)")
+        if (s.rows, s.consumed) != (d.rows, d.consumed) or not torch.equal(s.head, d.head.to(self.device)):
+            raise ValueError("the draft must hold the same streams: prefill the same prompt")
+        if cfg.seed is not None:
+            self.rng.manual_seed(cfg.seed)
+        stops = self.stop_ids if cfg.stop_ids is None else tuple(cfg.stop_ids)
+        stop_t = torch.tensor(stops, dtype=torch.int64, device=self.device) if stops else None
+        finished = torch.zeros(s.rows, dtype=torch.bool, device=self.device)
+        self.stop_reason = "max_new_tokens"
+        out, made = [], 0
+
+        def rand(*shape):
+            return torch.rand(*shape, generator=self.rng, device=self.device)
+
+        while made < cfg.max_new_tokens:
+            room = min(s.capacity, d.capacity) - s.consumed
+            if room <= 0:
+                self.stop_reason = "capacity"
+                break
+            K = min(n_draft, cfg.max_new_tokens - made - 1, room - 1)
+            guess, q = [], []
+            none = torch.empty(s.rows, 0, device=self.device)
+            tok = s.head
+            for _ in range(K):
+                q.append(probabilities(draft._consume(tok[:, None].to(draft.device), logits=True)[:, -1], cfg)
+                         .to(self.device))
+                tok = ops.verify_draft(q[-1][:, None], None, none.long(), none, rand(s.rows))[0][:, 0]
+                guess.append(tok)
+            tokens = torch.stack(guess, 1) if K else none.long()
+            p = probabilities(self._consume(torch.cat([s.head[:, None], tokens], 1), logits=True), cfg)
+            got, accepted = ops.verify_draft(p, torch.stack(q, 1) if K else None, tokens, rand(s.rows, K), rand(s.rows))
+            m = int(accepted.min()) if K else 0                 # the one host read per call of the model
+            stop = False
+            if stop_t is not None:
+                ended = torch.isin(got[:, :m + 1], stop_t).cumsum(1).bool() | finished[:, None]
+                over = ended.all(0).tolist()
+                if any(over):
+                    m, stop = over.index(True), True
+                finished = ended[:, m]
+            # both states keep the head and m accepted drafts; the newest token is the head again
+            self._rewind(K - m)
+            if m == K:
+                draft._consume((tokens[:, -1:] if K else s.head[:, None]).to(draft.device), logits=False)
+            else:
+                draft._rewind(K - 1 - m)
+            s.head = got[:, m].clone()
+            d.head = s.head.to(draft.device)
+            out.append(got[:, :m + 1])
+            made += m + 1
+            if stop:
+                self.stop_reason = "stop_id"
+                break
+        if not out:
+            return torch.empty(s.rows, 0, dtype=torch.int64, device=self.device)
+        return torch.cat(out, 1)
 
     def generate_ids(self, ids: torch.Tensor, cfg: SamplingConfig, max_len: int | None = None) -> torch.Tensor:
         """Fresh streams, ``ids`` as the prompt, the completion out."""

@@ -4,7 +4,8 @@ conv on q/k/v, per-head qk RMSNorm before RoPE, optional sigmoid output gate.
 On CUDA the training forward runs the fused qk-norm + RoPE kernel and the
 sm_100a flash-attention kernels (``vagus_b200.ops.attention``); decode with a
 KV cache uses the same kernels with a lower-right causal mask (query i sits at
-absolute position offset + i).  ``max_attn_logit`` is a probe (fp32, full
+absolute position offset + i).  ``set_cache_bits(4)`` holds the cache in 4 bits
+(``ops.Int4KV``) and decodes with ``ops.int4_attention``.  ``max_attn_logit`` is a probe (fp32, full
 score matrix, small inputs only).
 
 Parity: reference ``infra/components/attention.py:16-382``.
@@ -68,6 +69,8 @@ class SoftmaxAttention(nn.Module, Mixer):
         if out_proj:
             nn.init.normal_(self.wo.weight, std=init_std / math.sqrt(2 * layer_count) if layer_count else init_std)
         self.cache_len = 0
+        self.cache_bits = 16              # 16: the compute dtype; 4: Int4KV
+        self.kv4: ops.Int4KV | None = None
         self.register_buffer("k_cache", torch.zeros(0, 0, 0, 0), persistent=False)
         self.register_buffer("v_cache", torch.zeros(0, 0, 0, 0), persistent=False)
         if short_conv_size is not None:
@@ -93,6 +96,9 @@ class SoftmaxAttention(nn.Module, Mixer):
         qn = self.q_norm.gamma if self.qk_norm else None
         kn = self.k_norm.gamma if self.qk_norm else None
         eps = self.q_norm.eps if self.qk_norm else 1e-6
+        if self.rope is not None and not self.rope.table_form:
+            q, k = self.rope.rotate(ops.qk_norm_rope(q, qn, None, eps), ops.qk_norm_rope(k, kn, None, eps), offset)
+            return q.transpose(1, 2), k.transpose(1, 2)
         tables = self.rope.tables(L, offset) if self.rope is not None else None
         q = ops.qk_norm_rope(q, qn, tables, eps)
         k = ops.qk_norm_rope(k, kn, tables, eps)
@@ -136,12 +142,26 @@ class SoftmaxAttention(nn.Module, Mixer):
 
     # --- streaming ---------------------------------------------------------
 
+    def set_cache_bits(self, bits: int) -> None:
+        """16: keys and values cached in the compute dtype; 4: in 4 bits
+        (``ops.Int4KV``; head dims in multiples of 32).  Takes effect at the next
+        ``reset_cache`` / ``load_cache``."""
+        if bits not in (4, 16):
+            raise ValueError(f"cache_bits must be 4 or 16, got {bits}")
+        if bits == 4 and (self.head_dim % 32 or self.value_head_dim % 32):
+            raise ValueError(f"a 4-bit cache needs head dims in multiples of 32, got {self.head_dim} and "
+                             f"{self.value_head_dim}")
+        self.cache_bits = bits
+
     def reset_cache(self, batch_size: int, max_cache_len: int):
         device, dtype = infer_device(self), infer_dtype(self)
         Hk, Dh, Dvh = self.kv_head_count, self.head_dim, self.value_head_dim
         self.cache_len = 0
-        self.k_cache = torch.zeros(batch_size, Hk, max_cache_len, Dh, device=device, dtype=dtype)
-        self.v_cache = torch.zeros(batch_size, Hk, max_cache_len, Dvh, device=device, dtype=dtype)
+        # with 4 bits the buffers hold no channels: they keep the batch, the capacity and the dtype
+        held = 0 if self.cache_bits == 4 else 1
+        self.k_cache = torch.zeros(batch_size, Hk, max_cache_len, held * Dh, device=device, dtype=dtype)
+        self.v_cache = torch.zeros(batch_size, Hk, max_cache_len, held * Dvh, device=device, dtype=dtype)
+        self.kv4 = None if held else ops.Int4KV.empty(batch_size, Hk, max_cache_len, Dh, Dvh, device=device)
         if self.short_conv_size is not None:
             K = self.short_conv_size
             self.qp_cache = torch.zeros(batch_size, K, self.dim, device=device, dtype=dtype)
@@ -151,25 +171,46 @@ class SoftmaxAttention(nn.Module, Mixer):
             self.rope.prepare_m(max_cache_len)
 
     def load_cache(self, cache: dict, max_cache_len: int):
-        prefix = cache["k_cache"].shape[2]
+        if ("kv4" in cache) != (self.cache_bits == 4):
+            raise ValueError(f"The cache was exported with another cache_bits than this layer's {self.cache_bits}.")
+        rows, prefix = (cache["kv4"][0] if "kv4" in cache else cache["k_cache"]).shape[0:3:2]
         if prefix > max_cache_len:
             raise ValueError("The cache length already exceeds the given max_cache_len.")
-        self.reset_cache(cache["k_cache"].shape[0], max_cache_len)
+        self.reset_cache(rows, max_cache_len)
         self.cache_len = prefix
-        self.k_cache[:, :, :prefix].copy_(cache["k_cache"])
-        self.v_cache[:, :, :prefix].copy_(cache["v_cache"])
+        if self.kv4 is not None:
+            for have, saved in zip(self.kv4.tensors(), cache["kv4"]):
+                have[:, :, :prefix].copy_(saved)
+        else:
+            self.k_cache[:, :, :prefix].copy_(cache["k_cache"])
+            self.v_cache[:, :, :prefix].copy_(cache["v_cache"])
         if self.short_conv_size is not None:
             self.qp_cache.copy_(cache["qp_cache"])
             self.kp_cache.copy_(cache["kp_cache"])
             self.vp_cache.copy_(cache["vp_cache"])
 
     def export_cache(self) -> dict:
-        out = {"k_cache": self.k_cache[:, :, :self.cache_len].clone(),
-               "v_cache": self.v_cache[:, :, :self.cache_len].clone()}
+        if self.kv4 is not None:
+            out = {"kv4": [t[:, :, :self.cache_len].clone() for t in self.kv4.tensors()]}
+        else:
+            out = {"k_cache": self.k_cache[:, :, :self.cache_len].clone(),
+                   "v_cache": self.v_cache[:, :, :self.cache_len].clone()}
         if self.short_conv_size is not None:
             out.update(qp_cache=self.qp_cache.clone(), kp_cache=self.kp_cache.clone(),
                        vp_cache=self.vp_cache.clone())
         return out
+
+    def can_rewind(self) -> bool:
+        """Whether the state can drop its newest tokens (a short conv's window cannot)."""
+        return self.short_conv_size is None
+
+    def rewind_cache(self, tokens: int) -> None:
+        """Drop the newest ``tokens`` tokens of the cache."""
+        if not self.can_rewind():
+            raise ValueError("a layer with a short conv cannot be rewound")
+        if not 0 <= tokens <= self.cache_len:
+            raise ValueError(f"cannot rewind {tokens} of {self.cache_len} tokens")
+        self.cache_len -= tokens
 
     @torch.no_grad()
     def decode_step(self, x):
@@ -180,6 +221,8 @@ class SoftmaxAttention(nn.Module, Mixer):
         assert B == self.k_cache.shape[0], "The input batch_size does not match with the cache."
         offset = self.cache_len
         T = offset + L
+        if L == 0:
+            return x.new_zeros(B, 0, self.dim if self.out_proj else self.out_width)
         assert T <= self.k_cache.shape[2], "Cache overflow. Allocate with a larger max_cache_len."
         qp, kp, vp = ops.linear(x, self.wq.weight), ops.linear(x, self.wk.weight), ops.linear(x, self.wv.weight)
         if self.short_conv_size is not None:
@@ -195,10 +238,14 @@ class SoftmaxAttention(nn.Module, Mixer):
             vp = self.conv_v.direct_conv(vp)[:, -L:]
         q, k = self._qk(qp, kp, offset)
         v = vp.reshape(B, L, self.kv_head_count, self.value_head_dim).transpose(1, 2)
-        self.k_cache[:, :, offset:T].copy_(k)
-        self.v_cache[:, :, offset:T].copy_(v)
+        if self.kv4 is not None:
+            ops.int4_append(self.kv4, k, v, offset)
+            out = ops.int4_attention(q, self.kv4, T)
+        else:
+            self.k_cache[:, :, offset:T].copy_(k)
+            self.v_cache[:, :, offset:T].copy_(v)
+            out = ops.attention(q, self.k_cache[:, :, :T], self.v_cache[:, :, :T], causal=True)
         self.cache_len = T
-        out = ops.attention(q, self.k_cache[:, :, :T], self.v_cache[:, :, :T], causal=True)
         out = out.transpose(1, 2).reshape(B, L, -1)
         if self.out_gate:
             out = ops.sigmoid_gate(out, ops.linear(x, self.wg.weight))

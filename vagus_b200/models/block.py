@@ -61,6 +61,12 @@ class Block(nn.Module, WithCache):
     def export_cache(self) -> dict:
         return {"att": self.att.export_cache()}
 
+    def can_rewind(self) -> bool:
+        return getattr(self.att, "can_rewind", lambda: False)()
+
+    def rewind_cache(self, tokens: int) -> None:
+        self.att.rewind_cache(tokens)
+
     @torch.no_grad()
     def decode_step(self, x):
         x = x + self.att.decode_step(self.rmsnorm1(x))

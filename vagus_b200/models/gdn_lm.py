@@ -25,7 +25,7 @@ from .kalman import KalmanDeltaNet
 from .lm import CausalLM
 from .mixer import Mixer
 from .parallel_mixer import ParallelMixer
-from .rope import RoPE
+from .rope import RoPE, rope_options
 from .scans import chunk_scan_flops
 
 KINDS = ("gdn", "softmax", "parallel")
@@ -44,7 +44,8 @@ class GDNLM(CausalLM):
                  layer_kinds: list[str] | None = None, softmax_head_dim: int = 64, softmax_rope: bool = True,
                  softmax_out_gate: bool = False, parallel_width: int | None = None, context_len: int = 2048,
                  rope_base: float = 10000, rmsnorm_eps: float = 1e-6, tie_embedding: bool = True,
-                 gate_proj_optimizer: str = "adamw"):
+                 gate_proj_optimizer: str = "adamw", rope_dim: int | None = None, rope_layout: str = "interleaved",
+                 rope_scaling: dict | None = None):
         super().__init__()
         assert gate_proj_optimizer in ("adamw", "muon")
         self.config: dict[str, Any] = dict(
@@ -57,7 +58,8 @@ class GDNLM(CausalLM):
             layer_pattern=layer_pattern, layer_kinds=layer_kinds, softmax_head_dim=softmax_head_dim,
             softmax_rope=softmax_rope, softmax_out_gate=softmax_out_gate, parallel_width=parallel_width,
             context_len=context_len, rope_base=rope_base, rmsnorm_eps=rmsnorm_eps,
-            tie_embedding=tie_embedding, gate_proj_optimizer=gate_proj_optimizer)
+            tie_embedding=tie_embedding, gate_proj_optimizer=gate_proj_optimizer,
+            **rope_options(rope_dim, rope_layout, rope_scaling))
 
         if layer_kinds is not None:
             kinds = [k.strip() for k in layer_kinds]
@@ -80,7 +82,8 @@ class GDNLM(CausalLM):
         self.rope = None
         if any(k != "gdn" for k in kinds) and softmax_rope:
             assert dim % softmax_head_dim == 0
-            self.rope = RoPE(dim, softmax_head_dim, context_len, base=rope_base)
+            self.rope = RoPE(dim, softmax_head_dim, context_len, base=rope_base, rotary_dim=rope_dim,
+                             layout=rope_layout, scaling=rope_scaling)
 
         assert write in WRITES, f"write must be one of {WRITES}, got {write!r}"
         self.write = write

@@ -16,6 +16,7 @@ import torch
 from torch import nn
 
 from .. import ops
+from .attention import SoftmaxAttention
 from .decodable import Decodable
 from .norm import RMSNorm
 
@@ -69,6 +70,33 @@ class CausalLM(nn.Module, Decodable):
 
     def export_cache(self) -> dict:
         return {"blocks": [blk.export_cache() for blk in self.blocks]}
+
+    def set_cache_bits(self, bits: int) -> None:
+        """Bits a value of every softmax layer's KV cache (16 or 4); takes effect
+        at the next ``reset_cache`` / ``load_cache``.  Recurrent states keep theirs."""
+        layers = [m for m in self.modules() if isinstance(m, SoftmaxAttention)]
+        if not layers:
+            raise ValueError("this model has no softmax layer, so no KV cache")
+        before = [m.cache_bits for m in layers]
+        try:
+            for m in layers:
+                m.set_cache_bits(bits)
+        except ValueError:
+            for m, old in zip(layers, before):
+                m.cache_bits = old
+            raise
+
+    def can_rewind(self) -> bool:
+        """Whether the streams can drop their newest tokens: softmax layers
+        without a short conv can, recurrent states cannot."""
+        return all(blk.can_rewind() for blk in self.blocks)
+
+    def rewind_cache(self, tokens: int) -> None:
+        """Drop the newest ``tokens`` tokens of every stream."""
+        if not self.can_rewind():
+            raise ValueError("this model's state cannot be rewound (a recurrent layer or a short conv)")
+        for blk in self.blocks:
+            blk.rewind_cache(tokens)
 
     @torch.no_grad()
     def decode_step(self, tokens, return_logits: bool = True):

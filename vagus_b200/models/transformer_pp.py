@@ -13,22 +13,24 @@ from torch import nn
 from .attention import SoftmaxAttention
 from .block import Block
 from .lm import CausalLM
-from .rope import RoPE
+from .rope import RoPE, rope_options
 
 
 class TransformerPP(CausalLM):
     def __init__(self, vocab_size: int, dim: int, head_dim: int, context_len: int, layer_count: int,
                  ffn_hidden_dim: int | None = None, kv_head_count: int | None = None,
                  rmsnorm_eps: float = 1e-6, rope_base: float = 10000, tie_embedding: bool = True,
-                 qk_norm: bool = False):
+                 qk_norm: bool = False, rope_dim: int | None = None, rope_layout: str = "interleaved",
+                 rope_scaling: dict | None = None):
         super().__init__()
         self.config: dict[str, Any] = dict(
             vocab_size=vocab_size, dim=dim, head_dim=head_dim, context_len=context_len,
             layer_count=layer_count, ffn_hidden_dim=ffn_hidden_dim, kv_head_count=kv_head_count,
-            rmsnorm_eps=rmsnorm_eps, rope_base=rope_base, tie_embedding=tie_embedding, qk_norm=qk_norm)
+            rmsnorm_eps=rmsnorm_eps, rope_base=rope_base, tie_embedding=tie_embedding, qk_norm=qk_norm, **rope_options(rope_dim, rope_layout, rope_scaling))
         assert dim % head_dim == 0
         self.embedding = nn.Embedding(vocab_size, dim)
-        self.rope = RoPE(dim, head_dim, context_len, base=rope_base)
+        self.rope = RoPE(dim, head_dim, context_len, base=rope_base, rotary_dim=rope_dim, layout=rope_layout,
+                         scaling=rope_scaling)
         heads = dim // head_dim
         self.blocks = nn.ModuleList([
             Block(dim=dim, ffn_hidden_dim=ffn_hidden_dim, rmsnorm_eps=rmsnorm_eps, layer_count=layer_count,

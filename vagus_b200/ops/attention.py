@@ -147,12 +147,14 @@ class _AttnLayer(torch.autograd.Function):
 
 def attention_layer_ok(m, x) -> bool:
     """Whether the fused projection + attention path takes this layer and input:
-    CUDA, bf16 compute, no short conv or output gate, head dims 64 / 128 and
-    GEMM-sized projections."""
+    CUDA, bf16 compute, no short conv or output gate, RoPE (if any) from
+    tables, head dims 64 / 128 and GEMM-sized projections."""
     from .linear import gemm_ok
     if not (x.is_cuda and x.dim() == 3 and hasattr(native(), "attn_fwd")):
         return False
     if m.short_conv_size is not None or m.out_gate:
+        return False
+    if m.rope is not None and not m.rope.table_form:
         return False
     if not (x.dtype == torch.bfloat16 or autocast_bf16()):
         return False

@@ -131,7 +131,7 @@ def int4_attention_ref(q, k, v, lengths, causal: bool = True):
     p = torch.exp(s - torch.where(top == float("-inf"), torch.zeros_like(top), top))
     total = p.sum(-1, keepdim=True)
     p = p / torch.where(total == 0, torch.ones_like(total), total)     # a row that sees nothing gives zeros
-    return (p.view(B, Hk, H // Hk * Lq, T) @ v).view(B, H, Lq, -1).to(q.dtype)
+    return (p.view(B, Hk, H // Hk * Lq, T) @ v).view(B, H, Lq, v.shape[-1]).to(q.dtype)
 
 
 # ------------------------------------------------------------------ entry points --
