@@ -1,5 +1,6 @@
 // Bindings of the flash-attention kernels (attention.cu).
 #include <torch/extension.h>
+#include <string>
 #include <ATen/cuda/CUDAContext.h>
 
 #include "kernels.h"
@@ -13,7 +14,7 @@ using torch::Tensor;
 cudaStream_t stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 
 void check(int rc, const char* what) {
-  TORCH_CHECK(rc == 0, "vagus_b200 kernel '", what, "' rejected the problem or failed to launch (code ", rc, ")");
+  TORCH_CHECK(rc == 0, "vagus_b200 kernel '", what, "' rejected the problem or failed to launch (code ", std::to_string(rc), ")");
 }
 
 vagus::AttnArgs make_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& lse,

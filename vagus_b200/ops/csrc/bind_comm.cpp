@@ -75,7 +75,7 @@ void comm_all_gather(Tensor out, std::vector<int64_t> bases, int64_t rank, int64
   const int rc = vagus::comm_all_gather(peers_of(bases), static_cast<int>(rank), world, static_cast<unsigned>(epoch),
                                         out.data_ptr(), total / world, slot_cap, g_peer_wait_ns, vagus_device_error_ptr(),
                                         stream());
-  TORCH_CHECK(rc == 0, "comm_all_gather failed (code ", rc, ")");
+  TORCH_CHECK(rc == 0, "comm_all_gather failed (code ", std::to_string(rc), ")");
 }
 
 // in (world * n), out (n), same dtype (fp32 or bf16): out = scale * sum_r in_r[rank * n : rank * n + n]
@@ -90,7 +90,7 @@ void comm_reduce_scatter(Tensor out, Tensor in, std::vector<int64_t> bases, int6
                                             static_cast<unsigned>(epoch), in.data_ptr(), out.data_ptr(), out.numel(),
                                             static_cast<int>(in.element_size()), static_cast<float>(scale), ag_cap,
                                             slot_cap, g_peer_wait_ns, vagus_device_error_ptr(), stream());
-  TORCH_CHECK(rc == 0, "comm_reduce_scatter failed (code ", rc, ")");
+  TORCH_CHECK(rc == 0, "comm_reduce_scatter failed (code ", std::to_string(rc), ")");
 }
 
 // In-place NVLink all-reduce of a contiguous fp32 / bf16 tensor, times scale
@@ -103,7 +103,7 @@ void comm_all_reduce(Tensor buf, std::vector<int64_t> bases, int64_t rank, int64
                                         static_cast<unsigned>(epoch), buf.data_ptr(), buf.numel(),
                                         static_cast<int>(buf.element_size()), static_cast<float>(scale), slot_cap,
                                         g_peer_wait_ns, vagus_device_error_ptr(), stream());
-  TORCH_CHECK(rc == 0, "comm_all_reduce failed (code ", rc, ")");
+  TORCH_CHECK(rc == 0, "comm_all_reduce failed (code ", std::to_string(rc), ")");
 }
 
 // Epoch barrier over the heaps (the generic flag block).
@@ -111,7 +111,7 @@ void comm_barrier(std::vector<int64_t> bases, int64_t rank, int64_t epoch) {
   const int rc = vagus::comm_barrier(peers_of(bases), static_cast<int>(rank), static_cast<int>(bases.size()),
                                      vagus::kCommBarFlags, static_cast<unsigned>(epoch), g_peer_wait_ns,
                                      vagus_device_error_ptr(), stream());
-  TORCH_CHECK(rc == 0, "comm_barrier failed (code ", rc, ")");
+  TORCH_CHECK(rc == 0, "comm_barrier failed (code ", std::to_string(rc), ")");
 }
 
 // Push the blocks of a contiguous tensor to their owners' heaps (see comm.cu).
@@ -122,7 +122,7 @@ void comm_scatter_blocks(std::vector<int64_t> bases, int64_t slot_off, Tensor sr
   const int rc = vagus::comm_scatter_blocks(peers_of(bases), static_cast<int>(bases.size()), slot_off, src.data_ptr(),
                                             blk_bytes, static_cast<int>(nblk), static_cast<int>(per_rank), dst_stride,
                                             dst_off, stream());
-  TORCH_CHECK(rc == 0, "comm_scatter_blocks failed (code ", rc, ")");
+  TORCH_CHECK(rc == 0, "comm_scatter_blocks failed (code ", std::to_string(rc), ")");
 }
 
 // A tensor over `numel` elements of this process's heap at byte offset

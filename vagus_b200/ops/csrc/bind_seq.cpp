@@ -1,6 +1,7 @@
 // Bindings of the sequence-mixing kernels: short conv, gate activations,
 // the gated delta-rule recurrence and its decode step.
 #include <torch/extension.h>
+#include <string>
 #include <ATen/cuda/CUDAContext.h>
 
 #include "kernels.h"
@@ -14,7 +15,7 @@ using torch::Tensor;
 cudaStream_t stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 
 void check(int rc, const char* what) {
-  TORCH_CHECK(rc == 0, "vagus_b200 kernel '", what, "' failed to launch (code ", rc, ")");
+  TORCH_CHECK(rc == 0, "vagus_b200 kernel '", what, "' failed to launch (code ", std::to_string(rc), ")");
 }
 
 const float* fptr(const c10::optional<Tensor>& t) {

@@ -1,6 +1,7 @@
 // Python bindings of the sm_100a kernels.  Tensor checks live here; the .cu
 // files see raw pointers only.  Every op runs on the current CUDA stream.
 #include <torch/extension.h>
+#include <string>
 #include <vector>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -15,7 +16,7 @@ using torch::Tensor;
 cudaStream_t stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 
 void check(int rc, const char* what) {
-  TORCH_CHECK(rc == 0, "vagus_b200 kernel '", what, "' failed to launch (code ", rc, ")");
+  TORCH_CHECK(rc == 0, "vagus_b200 kernel '", what, "' failed to launch (code ", std::to_string(rc), ")");
 }
 
 bool is_f32(const Tensor& t) { return t.scalar_type() == at::kFloat; }
@@ -104,7 +105,7 @@ int64_t gemm(Tensor A, bool a_mn, Tensor B, bool b_mn, Tensor C, c10::optional<T
   g.K = static_cast<int>(a_mn ? ar : ac);
   g.N = static_cast<int>(b_mn ? bc : br);
   const int64_t kb = b_mn ? br : bc;
-  TORCH_CHECK(kb == g.K, "gemm: K mismatch (", g.K, " vs ", kb, ")");
+  TORCH_CHECK(kb == g.K, "gemm: K mismatch (", std::to_string(g.K), " vs ", std::to_string(kb), ")");
   TORCH_CHECK(C.size(-2) == g.M && C.size(-1) == g.N, "gemm: C shape mismatch");
   g.A = A.data_ptr(); g.B = B.data_ptr();
   g.lda = A.stride(-2); g.ldb = B.stride(-2);
