@@ -50,17 +50,22 @@ def test_rotary_gradient_against_differences(layout):
     assert torch.autograd.gradcheck(lambda a, b: ops.rotary(a, b, 5, frequencies(6), layout=layout, scale=0.7), (q, k))
 
 
-def test_rotary_refusals():
-    q, k, inv = torch.randn(2, 3, 4, 8), torch.randn(2, 3, 2, 8), frequencies(8)
+def rotary_refusals(device):
+    q, k, inv = (t.to(device) for t in (torch.randn(2, 3, 4, 8), torch.randn(2, 3, 2, 8), frequencies(8)))
     bad = [dict(layout="pairs"), dict(q=q[0]), dict(k=k[:, :2]), dict(k=k[..., :6]), dict(k=k.double()),
-           dict(inv=frequencies(10)), dict(inv=inv[:0]), dict(inv=inv.long()), dict(inv=inv[None]),
-           dict(pos=torch.arange(4)), dict(pos=torch.arange(3).float()), dict(pos=torch.zeros(3, 2).long()),
-           dict(pos=1.5)]
+           dict(inv=frequencies(10).to(device)), dict(inv=inv[:0]), dict(inv=inv.long()), dict(inv=inv[None]),
+           dict(inv=inv.to("meta")), dict(k=k.to("meta")),
+           dict(pos=torch.arange(4, device=device)), dict(pos=torch.arange(3, device=device).float()),
+           dict(pos=torch.zeros(3, 2, device=device).long()), dict(pos=torch.zeros(3, device="meta").long()), dict(pos=1.5)]
     for b in bad:
-        a = dict(q=q, k=k, pos=0, inv=inv, layout="half", **{})
+        a = dict(q=q, k=k, pos=0, inv=inv, layout="half")
         a.update(b)
         with pytest.raises(ValueError):
             ops.rotary(a["q"], a["k"], a["pos"], a["inv"], layout=a["layout"])
+
+
+def test_rotary_refusals():
+    rotary_refusals("cpu")
 
 
 # ------------------------------------------------------------------ 4-bit cache --
@@ -171,32 +176,51 @@ def test_attention_plain_form(H, Hk, Lq, causal):
     assert torch.allclose(same, got[2:3], atol=1e-6)
 
 
-def test_cache_refusals():
-    make = ops.Int4KV.empty
+def cache_refusals(device):
+    """On the GPU a place given there is checked by the kernel and does not raise here."""
+    def make(*a):
+        return ops.Int4KV.empty(*a, device=device)
+    here = device == "cpu"
+
+    def randn(*s):
+        return torch.randn(*s, device=device)
+
+    def places(*x):
+        return torch.tensor(x, device=device)
     for a in ((1, 1, 16, 48), (1, 1, 16, 0), (1, 1, 16, 64, 40)):
         with pytest.raises(ValueError):
             make(*a)
     c = make(2, 2, 16, 64, 32)
     kc, kp, vc, vp = c.tensors()
-    for t in ((kc[:, :, :8].contiguous(), kp[:, :, :8].contiguous(), vc[:, :, :8].contiguous(), vp[:, :, :8].contiguous()),
-              (kc.to(torch.int8), kp, vc, vp), (kc, kp.float(), vc, vp), (kc, vp, vc, vp), (kc[:1], kp[:1], vc, vp),
-              (kc.transpose(0, 1), kp, vc, vp), (kc[..., :20].contiguous(), kp, vc, vp)):
+    for t in ([x[:, :, :8].contiguous() for x in c.tensors()], (kc.to(torch.int8), kp, vc, vp), (kc, kp.float(), vc, vp),
+              (kc, vp, vc, vp), (kc[:1], kp[:1], vc, vp), (kc.transpose(2, 3), kp, vc, vp),
+              (kc[..., :20].contiguous(), kp, vc, vp), (kc, kp.flatten(3), vc, vp), (kc, kp, vc.to("meta"), vp)):
         with pytest.raises(ValueError):
             ops.Int4KV(*t)
-    k, v = torch.randn(2, 2, 3, 64), torch.randn(2, 2, 3, 32)
-    for a in ((k, v, 14), (k, v, -1), (k[:1], v, 0), (k, v[..., :16], 0), (k[:, :, :2], v, 0), (k.double(), v, 0),
-              (k, v, torch.tensor([0, 14])), (k, v, torch.tensor([-1, 0])), (k, v, torch.tensor([0])),
-              (k, v, torch.tensor([0.0, 1.0])), (k, v, 1.0)):
+    k, v = randn(2, 2, 3, 64), randn(2, 2, 3, 32)
+    bad = [(k, v, 14), (k, v, -1), (k[:1], v, 0), (k, v[..., :16], 0), (k[:, :, :2], v, 0), (k.double(), v, 0),
+           (k, v, places(0)), (k, v, places(0.0, 1.0)), (k, v, 1.0), (k, v, None), (k[0], v, 0), (k.to("meta"), v, 0)]
+    if here:
+        bad += [(k, v, places(0, 14)), (k, v, places(-1, 0))]
+    else:
+        bad += [(k.double(), v.double(), 0), (k, v, torch.tensor([0, 1]))]
+    for a in bad:
         with pytest.raises(ValueError):
             ops.int4_append(c, *a)
-    for a in ((0, 17), (-1, 2), (0, -1), (torch.tensor([0, 15]), 2)):
+    for a in ((0, 17), (-1, 2), (0, -1), (places(0, 1, 2), 2)) + (((places(0, 15), 2),) if here else ()):
         with pytest.raises(ValueError):
             ops.int4_read(c, *a)
-    q = torch.randn(2, 4, 1, 64)
-    for a in ((q, c, 17), (q, c, -1), (q[:1], c, 4), (q[:, :3], c, 4), (q[..., :32], c, 4), (q[0], c, 4),
-              (q, c, torch.tensor([4, 17])), (q, c, torch.tensor([4, 4, 4])), (q, c, None)):
+    assert all((t == 0).all() for t in c.tensors())
+    q = randn(2, 4, 1, 64).bfloat16()
+    bad = [(q, c, 17), (q, c, -1), (q[:1], c, 4), (q[:, :3], c, 4), (q[..., :32], c, 4), (q[0], c, 4),
+           (q, c, places(4, 4, 4)), (q, c, None), (q.to("meta"), c, 4)]
+    for a in bad + ([(q, c, places(4, 17))] if here else []):
         with pytest.raises(ValueError):
             ops.int4_attention(*a)
+
+
+def test_cache_refusals():
+    cache_refusals("cpu")
 
 
 # ----------------------------------------------------------------- verification --
@@ -301,13 +325,18 @@ def test_verify_special_rows():
         assert ops.verify_draft(one, None, torch.tensor([[d]]), u0, u1)[1].tolist() == [0]
 
 
-def test_verify_refusals():
-    target, draft, tokens, ua, us = drafted(2, 3, 5)
+def verify_refusals(device):
+    target, draft, tokens, ua, us = (t.to(device) for t in drafted(2, 3, 5))
     ok = dict(target=target, draft=draft, tokens=tokens, u_accept=ua, u_sample=us, lengths=None)
     for bad in (dict(target=target[0]), dict(target=target.double()), dict(target=target[:, :3]),
                 dict(draft=draft[:, :2]), dict(draft=draft.bfloat16()), dict(draft=draft[..., :4]),
                 dict(tokens=tokens.int()), dict(tokens=tokens[:1]), dict(u_accept=ua[:, :2]), dict(u_accept=ua.double()),
-                dict(u_sample=us[:1]), dict(u_sample=us[:, None]), dict(lengths=torch.zeros(3).long()),
-                dict(lengths=torch.zeros(2)), dict(target=target[..., :0], draft=draft[..., :0])):
+                dict(u_sample=us[:1]), dict(u_sample=us[:, None]), dict(lengths=torch.zeros(3, device=device).long()),
+                dict(lengths=torch.zeros(2, device=device)), dict(tokens=tokens.to("meta")), dict(u_sample=us.to("meta")),
+                dict(draft=draft.to("meta")), dict(tokens=tokens.reshape(-1)), dict(target=target[..., :0], draft=draft[..., :0])):
         with pytest.raises(ValueError):
             ops.verify_draft(**{**ok, **bad})
+
+
+def test_verify_refusals():
+    verify_refusals("cpu")

@@ -8,7 +8,8 @@ import pytest
 import torch
 
 from vagus_b200 import ops
-from tests.test_stream_ops import LAYOUTS, attention_64, drafted, frequencies, held_64, rotary_64, verify_64
+from tests.test_stream_ops import (LAYOUTS, attention_64, cache_refusals, drafted, frequencies, held_64,
+                                   rotary_64, rotary_refusals, verify_64, verify_refusals)
 
 pytestmark = pytest.mark.gpu
 
@@ -423,6 +424,11 @@ def test_verify_empty_batch():
     out, acc = ops.verify_draft(torch.empty(0, 4, 10, device=DEV), None, torch.empty(0, 3, device=DEV).long(),
                                 torch.empty(0, 3, device=DEV), torch.empty(0, device=DEV))
     assert out.shape == (0, 4) and acc.shape == (0,)
+
+
+@pytest.mark.parametrize("refusals", [rotary_refusals, cache_refusals, verify_refusals])
+def test_refusals(refusals):
+    refusals(DEV)
 
 
 # --------------------------------------------------------------------- together --

@@ -20,8 +20,6 @@ keys and values.  CUDA runs ``kv4.cu``; elsewhere the plain forms below run.
 from __future__ import annotations
 
 import math
-from dataclasses import dataclass
-
 import torch
 
 from ._core import native
@@ -30,31 +28,36 @@ GROUP = 32
 _BLOCK = 16         # the capacity is a whole number of blocks of this many tokens
 
 
-@dataclass
-class Int4KV:
-    """The four tensors of a cache, all contiguous on one device: codes
-    (B, Hk, capacity, D / 2) uint8 and parameters (B, Hk, capacity, D / 32, 2)
-    bf16 holding (s, b), for keys and for values."""
-    k_codes: torch.Tensor
-    k_params: torch.Tensor
-    v_codes: torch.Tensor
-    v_params: torch.Tensor
+def _check_cache(k_codes, k_params, v_codes, v_params) -> None:
+    for codes, params, what in ((k_codes, k_params, "k"), (v_codes, v_params, "v")):
+        if codes.dim() != 4 or codes.dtype != torch.uint8 or not codes.is_contiguous() \
+                or codes.shape[3] % (GROUP // 2) or not codes.shape[3]:
+            raise ValueError(f"Int4KV: {what}_codes must be (B, Hk, capacity, D / 2) uint8, contiguous, "
+                             f"D a multiple of {GROUP}")
+        want = (*codes.shape[:3], codes.shape[3] * 2 // GROUP, 2)
+        if tuple(params.shape) != want or params.dtype != torch.bfloat16 or not params.is_contiguous():
+            raise ValueError(f"Int4KV: {what}_params must be {want} bf16, contiguous")
+    if k_codes.shape[:3] != v_codes.shape[:3]:
+        raise ValueError("Int4KV: keys and values must agree in batch, heads and capacity")
+    if k_codes.shape[2] % _BLOCK:
+        raise ValueError(f"Int4KV: the capacity must be a multiple of {_BLOCK}")
+    if any(t.device != k_codes.device for t in (k_params, v_codes, v_params)):
+        raise ValueError("Int4KV: the tensors must be on one device")
 
-    def __post_init__(self):
-        for codes, params, what in ((self.k_codes, self.k_params, "k"), (self.v_codes, self.v_params, "v")):
-            if codes.dim() != 4 or codes.dtype != torch.uint8 or not codes.is_contiguous() \
-                    or codes.shape[3] % (GROUP // 2) or not codes.shape[3]:
-                raise ValueError(f"Int4KV: {what}_codes must be (B, Hk, capacity, D / 2) uint8, contiguous, "
-                                 f"D a multiple of {GROUP}")
-            want = (*codes.shape[:3], codes.shape[3] * 2 // GROUP, 2)
-            if tuple(params.shape) != want or params.dtype != torch.bfloat16 or not params.is_contiguous():
-                raise ValueError(f"Int4KV: {what}_params must be {want} bf16, contiguous")
-        if self.k_codes.shape[:3] != self.v_codes.shape[:3]:
-            raise ValueError("Int4KV: keys and values must agree in batch, heads and capacity")
-        if self.capacity % _BLOCK:
-            raise ValueError(f"Int4KV: the capacity must be a multiple of {_BLOCK}")
-        if any(t.device != self.k_codes.device for t in self.tensors()):
-            raise ValueError("Int4KV: the tensors must be on one device")
+
+class Int4KV:
+    """The four tensors of a cache, all contiguous (and 16-byte aligned) on one
+    device: codes (B, Hk, capacity, D / 2) uint8 and parameters
+    (B, Hk, capacity, D / 32, 2) bf16 holding (s, b), for keys and for values."""
+
+    __slots__ = ("k_codes", "k_params", "v_codes", "v_params")
+
+    def __init__(self, k_codes: torch.Tensor, k_params: torch.Tensor, v_codes: torch.Tensor, v_params: torch.Tensor):
+        if k_codes.is_cuda:
+            native().kv4_check(k_codes, k_params, v_codes, v_params)
+        else:
+            _check_cache(k_codes, k_params, v_codes, v_params)
+        self.k_codes, self.k_params, self.v_codes, self.v_params = k_codes, k_params, v_codes, v_params
 
     @classmethod
     def empty(cls, batch: int, kv_heads: int, capacity: int, head_dim: int, value_dim: int | None = None,
@@ -135,78 +138,91 @@ def int4_attention_ref(q, k, v, lengths, causal: bool = True):
 
 
 # ------------------------------------------------------------------ entry points --
+# On the GPU the bindings check the arguments, by the conditions written out here for the CPU.
 
-def _per_row(x, cache: Int4KV, what: str):
+def _place(x, what: str):
     """(tensor or None, int) of a place given as an int or per sequence."""
+    if isinstance(x, int):
+        return None, x
     if isinstance(x, torch.Tensor):
-        if x.dtype not in (torch.int32, torch.int64) or tuple(x.shape) != (cache.batch,) \
-                or x.device != cache.k_codes.device:
-            raise ValueError(f"{what} must be an int or ({cache.batch},) int32 / int64 on the cache's device")
-        return x.contiguous(), 0
-    if not isinstance(x, int):
-        raise ValueError(f"{what} must be an int or a tensor")
-    return None, x
+        return x, 0
+    raise ValueError(f"{what} must be an int or a tensor")
 
 
-def _rows(per, at, cache):
-    return per.to(torch.int64) if per is not None else torch.full((cache.batch,), at, device=cache.k_codes.device)
-
-
-def _span(cache: Int4KV, per, at: int, count: int, what: str):
-    """Host-side check of tokens [start, start + count)."""
+def _rows(per, at, cache: Int4KV, what: str):
+    """(B,) int64 places."""
     if per is None:
-        ok = 0 <= at and at + count <= cache.capacity
-    else:
-        # a start on the GPU is checked there (``check_error`` reports it)
-        ok = per.is_cuda or per.numel() == 0 or (int(per.min()) >= 0 and int(per.max()) + count <= cache.capacity)
-    if count < 0 or not ok:
+        return torch.full((cache.batch,), at, device=cache.k_codes.device)
+    if per.dtype not in (torch.int32, torch.int64) or tuple(per.shape) != (cache.batch,) \
+            or per.device != cache.k_codes.device:
+        raise ValueError(f"{what} must be an int or ({cache.batch},) int32 / int64 on the cache's device")
+    return per.to(torch.int64)
+
+
+def _span(cache: Int4KV, start, count: int, what: str) -> None:
+    if count < 0 or (start.numel() and (int(start.min()) < 0 or int(start.max()) + count > cache.capacity)):
         raise ValueError(f"{what}: tokens outside the cache of {cache.capacity}")
 
 
+def _at(cache: Int4KV, start, count: int):
+    """Indices of tokens start .. start + count - 1 in the cache's tensors."""
+    return (torch.arange(cache.batch)[:, None, None], torch.arange(cache.kv_heads)[None, :, None],
+            start[:, None, None] + torch.arange(count))
+
+
 @torch.no_grad()
-def int4_append(cache: Int4KV, k, v, start) -> None:
-    """Quantise ``k`` (B, Hk, L, D) and ``v`` (B, Hk, L, Dv) into the cache as
-    tokens start .. start + L - 1 (``start``: an int, or (B,) int32 / int64 for
-    a place per sequence; one given on the GPU is checked by the kernel, which
-    writes nothing outside the cache and reports it through ``check_error``)."""
+def _append_plain(cache, k, v, per, at):
     if k.dim() != 4 or v.dim() != 4 or k.shape[:3] != v.shape[:3] or k.shape[0] != cache.batch \
             or k.shape[1] != cache.kv_heads or k.shape[3] != cache.head_dim or v.shape[3] != cache.value_dim:
         raise ValueError(f"int4_append: k {tuple(k.shape)}, v {tuple(v.shape)} do not fit the cache")
     if k.dtype != v.dtype or k.device != cache.k_codes.device or v.device != cache.k_codes.device:
         raise ValueError("int4_append: k and v must share a dtype and be on the cache's device")
-    per, at = _per_row(start, cache, "int4_append: start")
-    L = k.shape[2]
-    _span(cache, per, at, L, "int4_append")
-    if k.is_cuda:
-        if k.dtype not in (torch.float32, torch.float16, torch.bfloat16):
-            raise ValueError(f"int4_append: {k.dtype} on the GPU (fp32, fp16 or bf16)")
-        k, v = (x if x.stride(-1) == 1 else x.contiguous() for x in (k, v))
-        native().kv4_append(*cache.tensors(), k, v, per, at)
-        return
-    i = torch.arange(cache.batch)[:, None, None]
-    j = torch.arange(cache.kv_heads)[None, :, None]
-    t = _rows(per, at, cache)[:, None, None] + torch.arange(L)
+    start = _rows(per, at, cache, "int4_append: start")
+    _span(cache, start, k.shape[2], "int4_append")
+    idx = _at(cache, start, k.shape[2])
     for have, new in zip(cache.tensors(), int4_quantise_ref(k) + int4_quantise_ref(v)):
-        have[i, j, t] = new
+        have[idx] = new
 
 
-@torch.no_grad()
+def int4_append(cache: Int4KV, k, v, start) -> None:
+    """Quantise ``k`` (B, Hk, L, D) and ``v`` (B, Hk, L, Dv) into the cache as
+    tokens start .. start + L - 1 (``start``: an int, or (B,) int32 / int64 for
+    a place per sequence; one given on the GPU is checked by the kernel, which
+    writes nothing outside the cache and reports it through ``check_error``).
+    fp32, fp16 or bf16 on the GPU."""
+    per, at = _place(start, "int4_append: start")
+    if cache.k_codes.is_cuda:
+        native().kv4_append(cache.k_codes, cache.k_params, cache.v_codes, cache.v_params, k, v, per, at)
+    else:
+        _append_plain(cache, k, v, per, at)
+
+
 def int4_read(cache: Int4KV, start, count: int):
     """The values of tokens start .. start + count - 1 as bf16 k (B, Hk, count, D)
     and v (B, Hk, count, Dv); ``start`` as in ``int4_append`` (tokens outside
     the cache read as zeros on the GPU and are reported)."""
-    per, at = _per_row(start, cache, "int4_read: start")
-    _span(cache, per, at, count, "int4_read")
+    per, at = _place(start, "int4_read: start")
     if cache.k_codes.is_cuda:
-        return tuple(native().kv4_read(*cache.tensors(), per, at, count))
-    i = torch.arange(cache.batch)[:, None, None]
-    j = torch.arange(cache.kv_heads)[None, :, None]
-    t = _rows(per, at, cache)[:, None, None] + torch.arange(count)
-    kc, kp, vc, vp = (x[i, j, t] for x in cache.tensors())
+        return native().kv4_read(cache.k_codes, cache.k_params, cache.v_codes, cache.v_params, per, at, count)
+    start = _rows(per, at, cache, "int4_read: start")
+    _span(cache, start, count, "int4_read")
+    idx = _at(cache, start, count)
+    kc, kp, vc, vp = (x[idx] for x in cache.tensors())
     return int4_values_ref(kc, kp), int4_values_ref(vc, vp)
 
 
 @torch.no_grad()
+def _attention_plain(q, cache, per, at, causal):
+    if q.dim() != 4 or q.shape[0] != cache.batch or q.shape[3] != cache.head_dim or not cache.kv_heads \
+            or q.shape[1] % cache.kv_heads or q.device != cache.k_codes.device:
+        raise ValueError(f"int4_attention: q {tuple(q.shape)} does not fit the cache")
+    lengths = _rows(per, at, cache, "int4_attention: lengths")
+    if not q.is_cuda and lengths.numel() and (int(lengths.max()) > cache.capacity or (per is None and at < 0)):
+        raise ValueError(f"int4_attention: lengths outside the cache of {cache.capacity}")
+    k, v = int4_read(cache, 0, cache.capacity if per is not None else at)
+    return int4_attention_ref(q, k, v, lengths.clamp(0, cache.capacity), causal)
+
+
 def int4_attention(q, cache: Int4KV, lengths, causal: bool = True):
     """Attention of ``q`` (B, H, Lq, D) over the first ``lengths`` tokens of the
     cache -> (B, H, Lq, Dv); H is a multiple of the cache's heads.
@@ -216,19 +232,11 @@ def int4_attention(q, cache: Int4KV, lengths, causal: bool = True):
     ``causal`` the queries are the last Lq of those tokens: query i sees the
     first lengths - Lq + i + 1 of them.  A query that sees nothing gives zeros.
     What the cache holds past a sequence's length has no effect.  Inference
-    only: no gradient flows."""
-    if q.dim() != 4 or q.shape[0] != cache.batch or q.shape[3] != cache.head_dim or not cache.kv_heads \
-            or q.shape[1] % cache.kv_heads:
-        raise ValueError(f"int4_attention: q {tuple(q.shape)} does not fit the cache")
-    if q.device != cache.k_codes.device:
-        raise ValueError("int4_attention: q must be on the cache's device")
-    per, at = _per_row(lengths, cache, "int4_attention: lengths")
-    if per is None:
-        if not 0 <= at <= cache.capacity:
-            raise ValueError(f"int4_attention: {at} tokens in a cache of {cache.capacity}")
-    elif not per.is_cuda and per.numel() and int(per.max()) > cache.capacity:
-        raise ValueError(f"int4_attention: lengths exceed the cache of {cache.capacity}")
-    if q.is_cuda and q.dtype == torch.bfloat16 and cache.head_dim in (64, 128) and cache.value_dim in (64, 128):
-        return native().kv4_attn(q, *cache.tensors(), per, at, bool(causal), 1.0 / math.sqrt(q.shape[-1]))
-    k, v = int4_read(cache, 0, cache.capacity if per is not None else at)
-    return int4_attention_ref(q, k, v, _rows(per, at, cache).clamp(0, cache.capacity), causal)
+    only: no gradient flows.  The kernels take bf16 queries and head dims 64 and
+    128; the plain form serves the others."""
+    per, at = _place(lengths, "int4_attention: lengths")
+    if cache.k_codes.is_cuda:
+        o = native().kv4_attn(q, cache.k_codes, cache.k_params, cache.v_codes, cache.v_params, per, at, causal)
+        if o is not None:
+            return o
+    return _attention_plain(q, cache, per, at, causal)

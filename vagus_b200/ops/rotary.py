@@ -16,6 +16,7 @@ import torch
 from ._core import native
 
 LAYOUTS = ("interleaved", "half")
+_KERNEL_TYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
 def _positions(positions, B, L, device):
@@ -42,10 +43,6 @@ def rotary_ref(x, positions, inv_freq, layout: str = "interleaved", scale: float
     return torch.cat((y.to(x.dtype), x[..., R:]), -1)
 
 
-def _unit(x):
-    return x if x is None or x.stride(-1) == 1 else x.contiguous()
-
-
 class _Rotary(torch.autograd.Function):
     """q and, unless it is None, k.  The backward applies this function with the
     angles negated, so it is differentiable itself."""
@@ -55,7 +52,7 @@ class _Rotary(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(pos, inv)
         ctx.meta = (offset, interleaved, scale, sign)
-        out = native().rotary(_unit(q), _unit(k), pos, offset, inv, interleaved, scale, sign)
+        out = native().rotary(q, k, pos, offset, inv, interleaved, scale, sign)
         return out[0], (out[1] if k is not None else None)
 
     @staticmethod
@@ -64,11 +61,33 @@ class _Rotary(torch.autograd.Function):
         offset, interleaved, scale, sign = ctx.meta
         if dq is None and dk is None:
             return (None,) * 8
+        run = _Rotary.apply if torch.is_grad_enabled() else _run
         if dq is None:
-            gk, gq = _Rotary.apply(dk, None, pos, offset, inv, interleaved, scale, -sign)
+            gk, gq = run(dk, None, pos, offset, inv, interleaved, scale, -sign)
         else:
-            gq, gk = _Rotary.apply(dq, dk, pos, offset, inv, interleaved, scale, -sign)
+            gq, gk = run(dq, dk, pos, offset, inv, interleaved, scale, -sign)
         return gq, gk, None, None, None, None, None, None
+
+
+def _run(q, k, *rest):
+    out = native().rotary(q, k, *rest)
+    return out if k is not None else (out[0], None)
+
+
+def _check(q, k, positions, inv_freq):
+    if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3])):
+        raise ValueError("rotary: q (B, L, H, D) and k (B, L, Hk, D)")
+    if k is not None and (k.dtype != q.dtype or k.device != q.device):
+        raise ValueError("rotary: q and k must share dtype and device")
+    B, L, D = q.shape[0], q.shape[1], q.shape[3]
+    if inv_freq.dim() != 1 or not inv_freq.is_floating_point() or not 1 <= inv_freq.shape[0] <= D // 2 \
+            or inv_freq.device != q.device:
+        raise ValueError(f"rotary: inv_freq (R/2,) on q's device with 2 <= R <= {D}")
+    if isinstance(positions, torch.Tensor):
+        if positions.dtype not in (torch.int32, torch.int64) or positions.device != q.device:
+            raise ValueError("rotary: positions must be int32 or int64 on q's device")
+        if tuple(positions.shape) not in ((L,), (B, L)):
+            raise ValueError(f"rotary: positions of shape ({L},) or ({B}, {L}), got {tuple(positions.shape)}")
 
 
 def rotary(q, k, positions, inv_freq, layout: str = "interleaved", scale: float = 1.0):
@@ -77,29 +96,21 @@ def rotary(q, k, positions, inv_freq, layout: str = "interleaved", scale: float 
 
     ``positions``: an int (token l sits at positions + l), or an int32 / int64
     tensor (L,) or (B, L).  ``inv_freq``: (R/2,) angle per step of position,
-    float64 (other float types are converted), R <= D."""
+    float64 (other float types are converted), R <= D.  Gradients flow to q and k."""
     if layout not in LAYOUTS:
         raise ValueError(f"rotary layout must be one of {LAYOUTS}, got {layout!r}")
-    if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3])):
-        raise ValueError("rotary: q (B, L, H, D) and k (B, L, Hk, D)")
-    if k is not None and (k.dtype != q.dtype or k.device != q.device):
-        raise ValueError("rotary: q and k must share dtype and device")
-    B, L, D = q.shape[0], q.shape[1], q.shape[3]
-    if inv_freq.dim() != 1 or not inv_freq.is_floating_point() or not 1 <= inv_freq.shape[0] <= D // 2:
-        raise ValueError(f"rotary: inv_freq (R/2,) with 2 <= R <= {D}")
-    if isinstance(positions, torch.Tensor):
-        if positions.dtype not in (torch.int32, torch.int64) or positions.device != q.device:
-            raise ValueError("rotary: positions must be int32 or int64 on q's device")
-        if tuple(positions.shape) not in ((L,), (B, L)):
-            raise ValueError(f"rotary: positions of shape ({L},) or ({B}, {L}), got {tuple(positions.shape)}")
-    elif not isinstance(positions, int):
+    if isinstance(positions, int):
+        pos, offset = None, positions
+    elif isinstance(positions, torch.Tensor):
+        pos, offset = positions, 0
+    else:
         raise ValueError("rotary: positions must be an int or a tensor")
-    if inv_freq.device != q.device:
-        raise ValueError("rotary: inv_freq must be on q's device")
-    if not q.is_cuda or q.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+    if not q.is_cuda or q.dtype not in _KERNEL_TYPES:
+        _check(q, k, positions, inv_freq)
         y = rotary_ref(q, positions, inv_freq, layout, scale)
         return y if k is None else (y, rotary_ref(k, positions, inv_freq, layout, scale))
-    pos, offset = (positions.expand(B, L), 0) if isinstance(positions, torch.Tensor) else (None, positions)
-    yq, yk = _Rotary.apply(q, k, pos, offset, inv_freq.detach().to(torch.float64).contiguous(), layout == "interleaved",
-                           float(scale), 1.0)
+    # on the GPU the binding checks the arguments (the same conditions)
+    graph = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
+    run = _Rotary.apply if graph else _run
+    yq, yk = run(q, k, pos, offset, inv_freq.detach(), layout == "interleaved", scale, 1.0)
     return yq if k is None else (yq, yk)

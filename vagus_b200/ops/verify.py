@@ -14,6 +14,7 @@ import torch
 from ._core import native
 
 
+@torch.no_grad()
 def verify_draft_ref(target, draft, tokens, u_accept, u_sample, lengths):
     B, K = tokens.shape
     V = target.shape[2]
@@ -48,22 +49,7 @@ def verify_draft_ref(target, draft, tokens, u_accept, u_sample, lengths):
     return out, accepted
 
 
-@torch.no_grad()
-def verify_draft(target, draft, tokens, u_accept, u_sample, lengths=None):
-    """``target`` (B, K + 1, V): the target's probabilities at the K drafted
-    places and the one after; ``draft`` (B, K, V): the probabilities the drafts
-    were drawn from, or None when they were certain (a lookup, a greedy draft:
-    q = 1, and a rejected token is struck out of p); ``tokens`` (B, K) int64;
-    ``u_accept`` (B, K) and ``u_sample`` (B,) fp32 in [0, 1); ``lengths`` (B,)
-    int32 / int64: drafted tokens of each row (default K).  fp32, fp16 or bf16
-    probabilities, which must be finite; they need not sum to one.
-
-    Returns ``(out, accepted)``: accepted (B,) int64, and out (B, K + 1) int64
-    holding the accepted drafts, the token that follows, then -1.  A drafted
-    token outside the vocabulary is rejected.  The next token is the first v
-    whose running sum of weights exceeds u_sample times their sum, in 64 bits;
-    where nothing is left of max(p - q, 0) it is drawn from p, and a row without
-    any weight gives token 0.  K = 0 draws one token from ``target``."""
+def _check(target, draft, tokens, u_accept, u_sample, lengths):
     if target.dim() != 3 or target.shape[1] < 1 or target.shape[2] < 1 \
             or target.dtype not in (torch.float32, torch.float16, torch.bfloat16):
         raise ValueError("verify_draft: target (B, K + 1, V), fp32, fp16 or bf16")
@@ -79,10 +65,24 @@ def verify_draft(target, draft, tokens, u_accept, u_sample, lengths=None):
         raise ValueError(f"verify_draft: lengths must be ({B},) int32 or int64")
     if any(t is not None and t.device != target.device for t in (draft, tokens, u_accept, u_sample, lengths)):
         raise ValueError("verify_draft: all tensors must be on one device")
-    if not target.is_cuda:
-        return verify_draft_ref(target, draft, tokens, u_accept, u_sample, lengths)
-    target = target if target.stride(2) == 1 else target.contiguous()
-    draft = draft if draft is None or draft.stride(2) == 1 else draft.contiguous()
-    lengths = None if lengths is None else lengths.contiguous()
-    out, accepted = native().verify_draft(target, draft, tokens, u_accept, u_sample, lengths)
-    return out, accepted
+
+
+def verify_draft(target, draft, tokens, u_accept, u_sample, lengths=None):
+    """``target`` (B, K + 1, V): the target's probabilities at the K drafted
+    places and the one after; ``draft`` (B, K, V): the probabilities the drafts
+    were drawn from, or None when they were certain (a lookup, a greedy draft:
+    q = 1, and a rejected token is struck out of p); ``tokens`` (B, K) int64;
+    ``u_accept`` (B, K) and ``u_sample`` (B,) fp32 in [0, 1); ``lengths`` (B,)
+    int32 / int64: drafted tokens of each row (default K).  fp32, fp16 or bf16
+    probabilities, which must be finite; they need not sum to one.
+
+    Returns ``(out, accepted)``: accepted (B,) int64, and out (B, K + 1) int64
+    holding the accepted drafts, the token that follows, then -1.  A drafted
+    token outside the vocabulary is rejected.  The next token is the first v
+    whose running sum of weights exceeds u_sample times their sum, in 64 bits;
+    where nothing is left of max(p - q, 0) it is drawn from p, and a row without
+    any weight gives token 0.  K = 0 draws one token from ``target``."""
+    if target.is_cuda:                       # the binding checks the arguments by the same conditions
+        return native().verify_draft(target, draft, tokens, u_accept, u_sample, lengths)
+    _check(target, draft, tokens, u_accept, u_sample, lengths)
+    return verify_draft_ref(target, draft, tokens, u_accept, u_sample, lengths)
