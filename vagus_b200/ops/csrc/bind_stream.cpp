@@ -215,16 +215,12 @@ c10::optional<Tensor> kv4_attn(Tensor q, Tensor kc, Tensor kp, Tensor vc, Tensor
   a.err = vagus_device_error_ptr();
   auto o = at::empty({c.B, q.size(2), q.size(1), c.Dv}, q.options());
   a.o = o.data_ptr();
-  a.splits = 1;
   Tensor part;
   if (o.numel() > 0) {
-    a.splits = vagus::kv4_attn_splits(a, a.lengths ? c.cap : length);
-    if (a.splits > 1) {
-      const int64_t rows = c.B * a.Lq * a.H * a.splits;
-      part = at::empty({rows * (c.Dv + 2)}, q.options().dtype(at::kFloat));
-      a.part_o = part.data_ptr<float>();
-      a.part_ml = a.part_o + rows * c.Dv;
-    }
+    vagus::kv4_attn_plan(a, a.lengths ? c.cap : length);
+    part = at::empty({a.part_rows * (c.Dv + 2)}, q.options().dtype(at::kFloat));
+    a.part_o = part.data_ptr<float>();
+    a.part_ml = a.part_o + a.part_rows * c.Dv;
     check(vagus::kv4_attn(a, at::cuda::getCurrentCUDAStream().stream()), "kv4_attn");
   }
   return o.transpose(1, 2);

@@ -126,10 +126,18 @@ __device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t 
   asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
   return d;
 }
+// The two constants of unpacking, from the kernel's arguments: the logic operation
+// takes one immediate at most, and with both known to the compiler each unpacking
+// costs two of them.
+struct Unpack {
+  uint32_t mask, magic;          // 0x000F000F, 0x43004300
+};
 // nibbles i and i + 4 of w (i = 0 .. 3) as the pair of values they stand for
 template <int I>
-__device__ __forceinline__ uint32_t pair_of(uint32_t w, uint32_t ss, uint32_t bb) {
-  return fma_bf16x2(((w >> (4 * I)) & 0x000F000Fu) | 0x43004300u, ss, bb);
+__device__ __forceinline__ uint32_t pair_of(uint32_t w, uint32_t ss, uint32_t bb, const Unpack& c) {
+  uint32_t x;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(x) : "r"(w >> (4 * I)), "r"(c.mask), "r"(c.magic));   // (w & mask) | magic
+  return fma_bf16x2(x, ss, bb);
 }
 __device__ __forceinline__ uint32_t low2(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x5410); }
 __device__ __forceinline__ uint32_t high2(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
@@ -155,17 +163,17 @@ __global__ void __launch_bounds__(256) kv4_read_k(const Kv4ReadArgs a) {
   const long long at = bh * a.cap + t;
   const uint32_t w = codes[at * per + cw], p = params[at * (D / kGroup) + cw / 4];
   const uint32_t ss = low2(p, p), bb = high2(p, p);
-  const uint32_t p0 = pair_of<0>(w, ss, bb), p1 = pair_of<1>(w, ss, bb), p2 = pair_of<2>(w, ss, bb),
-                 p3 = pair_of<3>(w, ss, bb);
+  const Unpack un{a.mask, a.magic};
+  const uint32_t p0 = pair_of<0>(w, ss, bb, un), p1 = pair_of<1>(w, ss, bb, un), p2 = pair_of<2>(w, ss, bb, un),
+                 p3 = pair_of<3>(w, ss, bb, un);
   out[i] = make_uint4(low2(p0, p1), low2(p2, p3), high2(p0, p1), high2(p2, p3));
 }
 
 // ------------------------------------------------------------- attention --
 //
-// One CTA of four warps per (split of the tokens, KV head and tile of query
-// rows, sequence).  The rows of a KV head are its Lq queries times the H / Hk
-// heads that share it; a tile has 8 NT of them, so one pass over the cache
-// serves them all.  Everything stays in registers:
+// The rows of a KV head are its Lq queries times the H / Hk heads that share it,
+// numbered query-major; a tile of 8 NT of them goes over the head's tokens once,
+// so one pass over the cache serves them all.  Everything stays in registers:
 //
 //   S^T (16 tokens x 8 rows)    += K (16 x 16 channels) q^T      mma m16n8k16
 //   O^T (16 channels x 8 rows)  += V^T (16 x 16 tokens) P^T
@@ -177,13 +185,26 @@ __global__ void __launch_bounds__(256) kv4_read_k(const Kv4ReadArgs a) {
 // leaves the product with a token a row; transposing the 8 x 8 tile of the
 // rounded probabilities (movmatrix) makes it the B operand of the second.
 //
-// Each warp has its own running maximum and sum over every fourth block of 32
-// tokens; the four meet in shared memory, the splits in a second kernel.
-// Probabilities are rounded to bf16 for the second product (2^-9 relative, the
-// size of the output's own rounding); scores, sums and accumulators are fp32.
+// The softmax's reference is raised only when a score exceeds it by 2^8: until
+// then probabilities above 1 do no harm (they keep their relative precision), and
+// a 16-token tile needs no reduction over its tokens.  Probabilities are rounded
+// to bf16 for the second product (2^-9 relative on average half of it, the size
+// of the output's own rounding); scores, sums and accumulators are fp32.
+//
+// Work.  An item is a row tile of one KV head of one sequence; its tokens are cut
+// into units of 128 (each of a CTA's four warps takes 32 of them).  All items'
+// units, laid end to end with two blank ones ahead of each item (what starting and
+// ending it costs), are dealt to the CTAs in equal contiguous shares, so ragged
+// batches and few long sequences fill the GPU alike.  A CTA writes the
+// items it has whole; of the first and last item of its share it may have a part,
+// which it leaves in slot 0 or 1 of its scratch, and the join kernel adds the
+// parts of an item in order.
 
 constexpr int kAttnWarps = 4;
-constexpr int kBlock = 32;            // tokens a warp takes at once
+constexpr int kUnit = 32 * kAttnWarps;      // tokens
+constexpr int kHead = 2;                    // what starting and ending an item costs, in units
+constexpr float kUnset = 1e30f;             // minus the softmax reference before the first score
+constexpr float kLazy = 8.f;                // raise the reference when a score exceeds it by so many powers of 2
 
 __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
   uint32_t d;
@@ -204,33 +225,57 @@ __device__ __forceinline__ void load_words(uint32_t (&r)[W], const uint8_t* p) {
   }
 }
 
-// the codes and parameters of 16 tokens that one lane works on
+// A lane's places in the tensors of one item, and the codes and parameters of the
+// 16 tokens that start `token` tokens further on.
 template <int D, int DV>
-struct Frag {
-  static constexpr int KW = D / 32, VW = DV / 64;
-  uint32_t k[2][KW], kp[2], v[4][VW], vp[4];
-
-  // t0: first token (a multiple of 16); the cache holds whole blocks of 16
-  __device__ __forceinline__ void load(const Kv4AttnArgs& a, long long bh, int t0, int g, int t) {
-    const long long at = bh * a.cap + t0;
+struct Keys {
+  static constexpr int W = D / 32;
+  const uint8_t *codes, *params;
+  __device__ __forceinline__ void at(const Kv4AttnArgs& a, long long row, int g, int t) {
+    codes = a.k_codes + (row + g) * (D / 2) + t * (4 * W);
+    params = static_cast<const uint8_t*>(a.k_params) + ((row + g) * (D / kGroup) + t * W / 4) * 4;
+  }
+  __device__ __forceinline__ void skip(int tokens) { codes += tokens * (D / 2); params += tokens * (D / kGroup * 4); }
+};
+template <int D, int DV>
+struct KeyFrag {
+  static constexpr int W = D / 32;
+  uint32_t w[2][W], p[2];
+  __device__ __forceinline__ void load(const Keys<D, DV>& k, int token) {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const long long row = at + g + 8 * r;
-      load_words<KW>(k[r], a.k_codes + row * (D / 2) + t * (4 * KW));
-      kp[r] = reinterpret_cast<const uint32_t*>(a.k_params)[row * (D / kGroup) + t * KW / 4];
-    }
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const long long row = at + 2 * t + (r & 1) + 8 * (r >> 1);
-      load_words<VW>(v[r], a.v_codes + row * (DV / 2) + g * (4 * VW));
-      vp[r] = reinterpret_cast<const uint32_t*>(a.v_params)[row * (DV / kGroup) + g * VW / 4];
+      load_words<W>(w[r], k.codes + (token + 8 * r) * (D / 2));
+      p[r] = *reinterpret_cast<const uint32_t*>(k.params + (token + 8 * r) * (D / kGroup * 4));
     }
   }
-  // tokens >= n stand for zero whatever the cache holds there
-  __device__ __forceinline__ void cut(int t0, int n, int t) {
+};
+template <int D, int DV>
+struct Values {
+  static constexpr int W = DV / 64;
+  const uint8_t *codes, *params;
+  __device__ __forceinline__ void at(const Kv4AttnArgs& a, long long row, int g, int t) {
+    codes = a.v_codes + (row + 2 * t) * (DV / 2) + g * (4 * W);
+    params = static_cast<const uint8_t*>(a.v_params) + ((row + 2 * t) * (DV / kGroup) + g * W / 4) * 4;
+  }
+  __device__ __forceinline__ void skip(int tokens) { codes += tokens * (DV / 2); params += tokens * (DV / kGroup * 4); }
+};
+template <int D, int DV>
+struct ValueFrag {
+  static constexpr int W = DV / 64;
+  uint32_t w[4][W], p[4];                  // tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+  __device__ __forceinline__ void load(const Values<D, DV>& v, int token) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int at = token + (r & 1) + 8 * (r >> 1);
+      load_words<W>(w[r], v.codes + at * (DV / 2));
+      p[r] = *reinterpret_cast<const uint32_t*>(v.params + at * (DV / kGroup * 4));
+    }
+  }
+  // of 16 tokens the first n stand for what they hold, the others for zero
+  __device__ __forceinline__ void cut(int n, int t) {
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      if (t0 + 2 * t + (r & 1) + 8 * (r >> 1) >= n) vp[r] = 0u;
+      if (2 * t + (r & 1) + 8 * (r >> 1) >= n) p[r] = 0u;
   }
 };
 
@@ -240,16 +285,18 @@ struct Query {
 };
 
 template <int D, int DV, int NT>
-__device__ __forceinline__ void scores_of(const Frag<D, DV>& f, const Query<D, NT>& q, float (&s)[NT][4]) {
+__device__ __forceinline__ void scores_of(const KeyFrag<D, DV>& f, const Query<D, NT>& q, float (&s)[NT][4], const Unpack& un) {
 #pragma unroll
   for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-  const uint32_t s0 = low2(f.kp[0], f.kp[0]), b0 = high2(f.kp[0], f.kp[0]);
-  const uint32_t s1 = low2(f.kp[1], f.kp[1]), b1 = high2(f.kp[1], f.kp[1]);
+  const uint32_t s0 = low2(f.p[0], f.p[0]), b0 = high2(f.p[0], f.p[0]);
+  const uint32_t s1 = low2(f.p[1], f.p[1]), b1 = high2(f.p[1], f.p[1]);
 #pragma unroll
   for (int w = 0; w < D / 32; ++w) {
-    const uint32_t x = f.k[0][w], y = f.k[1][w];
-    const uint32_t a0[4] = {pair_of<0>(x, s0, b0), pair_of<0>(y, s1, b1), pair_of<1>(x, s0, b0), pair_of<1>(y, s1, b1)};
-    const uint32_t a1[4] = {pair_of<2>(x, s0, b0), pair_of<2>(y, s1, b1), pair_of<3>(x, s0, b0), pair_of<3>(y, s1, b1)};
+    const uint32_t x = f.w[0][w], y = f.w[1][w];
+    const uint32_t a0[4] = {pair_of<0>(x, s0, b0, un), pair_of<0>(y, s1, b1, un), pair_of<1>(x, s0, b0, un),
+                            pair_of<1>(y, s1, b1, un)};
+    const uint32_t a1[4] = {pair_of<2>(x, s0, b0, un), pair_of<2>(y, s1, b1, un), pair_of<3>(x, s0, b0, un),
+                            pair_of<3>(y, s1, b1, un)};
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       mma::mma16816(s[n], a0, q.b[n][2 * w][0], q.b[n][2 * w][1]);
@@ -259,14 +306,16 @@ __device__ __forceinline__ void scores_of(const Frag<D, DV>& f, const Query<D, N
 }
 
 template <int D, int DV, int NT>
-__device__ __forceinline__ void add_values(const Frag<D, DV>& f, const uint32_t (&p)[NT][2], float (&o)[DV / 16][NT][4]) {
-  const uint32_t sl = low2(f.vp[0], f.vp[1]), bl = high2(f.vp[0], f.vp[1]);
-  const uint32_t sh = low2(f.vp[2], f.vp[3]), bh = high2(f.vp[2], f.vp[3]);
-  uint32_t xl[Frag<D, DV>::VW], yl[Frag<D, DV>::VW], xh[Frag<D, DV>::VW], yh[Frag<D, DV>::VW];
+__device__ __forceinline__ void add_values(const ValueFrag<D, DV>& f, const uint32_t (&p)[NT][2],
+                                           float (&o)[DV / 16][NT][4], const Unpack& un) {
+  constexpr int W = DV / 64;
+  const uint32_t sl = low2(f.p[0], f.p[1]), bl = high2(f.p[0], f.p[1]);
+  const uint32_t sh = low2(f.p[2], f.p[3]), bh = high2(f.p[2], f.p[3]);
+  uint32_t xl[W], yl[W], xh[W], yh[W];
 #pragma unroll
-  for (int w = 0; w < Frag<D, DV>::VW; ++w) {
-    xl[w] = low2(f.v[0][w], f.v[1][w]); yl[w] = high2(f.v[0][w], f.v[1][w]);
-    xh[w] = low2(f.v[2][w], f.v[3][w]); yh[w] = high2(f.v[2][w], f.v[3][w]);
+  for (int w = 0; w < W; ++w) {
+    xl[w] = low2(f.w[0][w], f.w[1][w]); yl[w] = high2(f.w[0][w], f.w[1][w]);
+    xh[w] = low2(f.w[2][w], f.w[3][w]); yh[w] = high2(f.w[2][w], f.w[3][w]);
   }
   auto product = [&](int i, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
     const uint32_t a[4] = {a0, a1, a2, a3};
@@ -276,16 +325,16 @@ __device__ __forceinline__ void add_values(const Frag<D, DV>& f, const uint32_t 
   if constexpr (DV == 128) {
     // product i: rows g are nibble i of word 2 g, rows g + 8 nibble i of word 2 g + 1
 #define VAGUS_KV4_V(I)                                                                                     \
-  product(I, pair_of<I>(xl[0], sl, bl), pair_of<I>(xl[1], sl, bl), pair_of<I>(xh[0], sh, bh),              \
-          pair_of<I>(xh[1], sh, bh));                                                                      \
-  product(I + 4, pair_of<I>(yl[0], sl, bl), pair_of<I>(yl[1], sl, bl), pair_of<I>(yh[0], sh, bh),          \
-          pair_of<I>(yh[1], sh, bh));
+  product(I, pair_of<I>(xl[0], sl, bl, un), pair_of<I>(xl[1], sl, bl, un), pair_of<I>(xh[0], sh, bh, un),              \
+          pair_of<I>(xh[1], sh, bh, un));                                                                      \
+  product(I + 4, pair_of<I>(yl[0], sl, bl, un), pair_of<I>(yl[1], sl, bl, un), pair_of<I>(yh[0], sh, bh, un),          \
+          pair_of<I>(yh[1], sh, bh, un));
     VAGUS_KV4_V(0) VAGUS_KV4_V(1) VAGUS_KV4_V(2) VAGUS_KV4_V(3)
 #undef VAGUS_KV4_V
   } else {
     // product i: rows g are nibble i of word g, rows g + 8 nibble i + 4
 #define VAGUS_KV4_V(I) \
-  product(I, pair_of<I>(xl[0], sl, bl), pair_of<I>(yl[0], sl, bl), pair_of<I>(xh[0], sh, bh), pair_of<I>(yh[0], sh, bh));
+  product(I, pair_of<I>(xl[0], sl, bl, un), pair_of<I>(yl[0], sl, bl, un), pair_of<I>(xh[0], sh, bh, un), pair_of<I>(yh[0], sh, bh, un));
     VAGUS_KV4_V(0) VAGUS_KV4_V(1) VAGUS_KV4_V(2) VAGUS_KV4_V(3)
 #undef VAGUS_KV4_V
   }
@@ -297,227 +346,341 @@ __device__ __forceinline__ int channel_of(int i, int g, int upper) {
   return DV == 128 ? 16 * g + 8 * upper + i : 8 * g + 4 * upper + i;
 }
 
+// The running softmax of a warp over the tokens it has seen, for its 8 NT rows.
 template <int D, int DV, int NT>
-__global__ void __launch_bounds__(32 * kAttnWarps) kv4_attn_k(const Kv4AttnArgs a) {
+struct Running {
+  float o[DV / 16][NT][4], l[NT][2], nref[NT][2];      // nref: minus the reference, in powers of 2
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      nref[j][0] = nref[j][1] = kUnset;
+      l[j][0] = l[j][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < DV / 16; ++i) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.f;
+    }
+  }
+
+  // raises the references to the largest scores of this tile where those are above
+  __device__ __forceinline__ void raise(const float (&s)[NT][4], float scale) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float mx = fmaxf(s[j][e], s[j][e + 2]);
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+        const float to = fminf(nref[j][e], -mx * scale), c = ex2_approx(to - nref[j][e]);
+        nref[j][e] = to;
+        l[j][e] *= c;
+#pragma unroll
+        for (int i = 0; i < DV / 16; ++i) {
+          o[i][j][e] *= c;
+          o[i][j][e + 2] *= c;
+        }
+      }
+  }
+
+  // scores -> probabilities against the references, added to the sums; as B operands in p
+  __device__ __forceinline__ void weigh(float (&s)[NT][4], float scale, uint32_t (&p)[NT][2]) {
+    float above = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) above = fmaxf(above, fmaf(s[j][e], scale, nref[j][e & 1]));
+    if (__any_sync(0xffffffffu, above > kLazy)) raise(s, scale);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[j][e] = ex2_approx(fmaf(s[j][e], scale, nref[j][e & 1]));
+        l[j][e & 1] += s[j][e];
+      }
+      p[j][0] = transpose8(pack_bf16x2(s[j][0], s[j][1]));
+      p[j][1] = transpose8(pack_bf16x2(s[j][2], s[j][3]));
+    }
+  }
+};
+
+__device__ __forceinline__ int length_of(const Kv4AttnArgs& a, long long b) {
+  long long n = a.lengths ? index_at(a.lengths, a.len_i64, b) : a.length;
+  if (n > a.cap) {
+    record_error(a.err, kErrBadArgument);
+    n = a.cap;
+  }
+  return n < 0 ? 0 : static_cast<int>(n);
+}
+// an empty sequence has one unit too: somebody writes its zeros
+__device__ __forceinline__ int units_of(int n) { return n <= kUnit ? 1 : (n + kUnit - 1) / kUnit; }
+
+// One warp: units (blank ones included) of all sequences (times `per` items each), and with
+// `flat` >= 0 the sequence that holds unit `flat` and the units before it.
+__device__ long long scan_units(const Kv4AttnArgs& a, int per, long long flat, long long& seq, long long& before) {
+  const int lane = threadIdx.x % 32;
+  if (a.lengths == nullptr) {
+    const long long u = static_cast<long long>(kHead + units_of(static_cast<int>(a.length))) * per;
+    if (flat >= 0) { seq = flat / u; before = seq * u; }
+    return u * a.B;
+  }
+  long long run = 0;
+  for (long long b0 = 0; b0 < a.B; b0 += 32) {
+    const long long b = b0 + lane;
+    const long long u = b < a.B ? static_cast<long long>(kHead + units_of(length_of(a, b))) * per : 0;
+    long long in = u;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long up = __shfl_up_sync(0xffffffffu, in, o);
+      if (lane >= o) in += up;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, flat >= 0 && run + in > flat);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      seq = b0 + src;
+      before = run + __shfl_sync(0xffffffffu, in - u, src);
+      return 0;
+    }
+    run += __shfl_sync(0xffffffffu, in, 31);
+  }
+  return run;
+}
+
+template <int D, int DV, int NT>
+__global__ void __launch_bounds__(32 * kAttnWarps, NT == 1 ? 3 : 2) kv4_attn_k(const Kv4AttnArgs a) {
   constexpr int ROWS = 8 * NT;
   __shared__ float sm[kAttnWarps][ROWS], sl[kAttnWarps][ROWS];
-  __shared__ float so[ROWS][DV + 4];
+  __shared__ float so[kAttnWarps][ROWS][DV + 4];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane >> 2, t = lane & 3;
-  const int split = blockIdx.x, hk = blockIdx.y % a.Hk, tile = blockIdx.y / a.Hk, G = a.H / a.Hk;
-  const long long b = blockIdx.z, bh = b * a.Hk + hk;
-  const int R = G * a.Lq, r0 = tile * ROWS;
+  const int G = a.H / a.Hk, R = G * a.Lq, tiles = (R + ROWS - 1) / ROWS, per = a.Hk * tiles;
 
-  long long len = a.lengths ? index_at(a.lengths, a.len_i64, b) : a.length;
-  if (len > a.cap) {
-    if (threadIdx.x == 0) record_error(a.err, kErrBadArgument);
-    len = a.cap;
-  }
-  const int n = len < 0 ? 0 : static_cast<int>(len);
+  long long seq = 0, before = 0;
+  const long long total = scan_units(a, per, -1, seq, before);
+  const long long share = (total + gridDim.x - 1) / gridDim.x;
+  long long u = blockIdx.x * share;
+  const long long end = min(total, u + share);
+  if (u >= end) return;
+  scan_units(a, per, u, seq, before);
+  bool first_of_share = true;
+  const Unpack un{a.mask, a.magic};
 
-  // rows are numbered query-major; a row sees the first `vis` tokens, the tile
-  // between `least` and `most`
-  const int first = r0 / G, last = (min(r0 + ROWS, R) - 1) / G;
-  const int least = a.causal ? max(0, n - a.Lq + 1 + first) : n;
-  const int most = a.causal ? max(0, n - a.Lq + 1 + last) : n;
-  int vis[NT][2];
+  long long seq_next = seq;
+  while (u < end) {
+    // the item that holds unit u, and the part of it that is this CTA's
+    const int n = length_of(a, seq), units = units_of(n);
+    const int item = static_cast<int>((u - before) / (kHead + units));
+    const long long item0 = before + static_cast<long long>(item) * (kHead + units) + kHead;
+    const int ua = static_cast<int>(max(0LL, u - item0)), ub = static_cast<int>(min(end - item0, static_cast<long long>(units)));
+    u = item0 + ub;
+    if (item + 1 == per && ub == units) {
+      before = u;
+      ++seq_next;
+    }
+    if (ub <= 0) break;                       // only blank units of it: the next CTA starts it
+    const int hk = item / tiles, r0 = (item - hk * tiles) * ROWS;
+    // a row sees the first `vis` tokens; the tile between `least` and `most`
+    const int first = r0 / G, last = (min(r0 + ROWS, R) - 1) / G;
+    const int least = a.causal ? max(0, n - a.Lq + 1 + first) : n;
+    const int most = a.causal ? max(0, n - a.Lq + 1 + last) : n;
+
+    Query<D, NT> q;
 #pragma unroll
-  for (int j = 0; j < NT; ++j)
+    for (int j = 0; j < NT; ++j) {
+      const int r = r0 + 8 * j + g;
+      const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(a.q) + seq * a.sq_b +
+                                 (hk * G + r % G) * a.sq_h + static_cast<long long>(r / G) * a.sq_l;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int r = r0 + 8 * j + 2 * t + e;
-      vis[j][e] = r < R && a.causal ? max(0, n - a.Lq + 1 + r / G) : most;
+      for (int w = 0; w < D / 32; ++w) {
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (r < R) x = *reinterpret_cast<const uint4*>(src + 8 * (t * (D / 32) + w));
+        q.b[j][2 * w][0] = low2(x.x, x.z);          // channels (0, 4)
+        q.b[j][2 * w][1] = high2(x.x, x.z);         // (1, 5)
+        q.b[j][2 * w + 1][0] = low2(x.y, x.w);      // (2, 6)
+        q.b[j][2 * w + 1][1] = high2(x.y, x.w);     // (3, 7)
+      }
     }
 
-  Query<D, NT> q;
-#pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    const int r = r0 + 8 * j + g;
-    const __nv_bfloat16* src =
-        static_cast<const __nv_bfloat16*>(a.q) + b * a.sq_b + (hk * G + r % G) * a.sq_h + (r / G) * a.sq_l;
-#pragma unroll
-    for (int w = 0; w < D / 32; ++w) {
-      uint4 u = make_uint4(0, 0, 0, 0);
-      if (r < R) u = *reinterpret_cast<const uint4*>(src + 8 * (t * (D / 32) + w));
-      q.b[j][2 * w][0] = low2(u.x, u.z);          // channels (0, 4)
-      q.b[j][2 * w][1] = high2(u.x, u.z);         // (1, 5)
-      q.b[j][2 * w + 1][0] = low2(u.y, u.w);      // (2, 6)
-      q.b[j][2 * w + 1][1] = high2(u.y, u.w);     // (3, 7)
+    Running<D, DV, NT> run;
+    run.clear();
+    // this warp's tiles of 16 tokens: two neighbouring ones of every unit, up to `most`
+    const int tile0 = 8 * ua + 2 * warp, tiles16 = (most + 15) / 16;
+    const int whole = (tiles16 - 2 * warp) / 8;                              // units with both tiles
+    int count = 0;
+    if (tiles16 > tile0) {
+      const int full = min(ub, max(0, whole)) - ua;
+      count = full > 0 ? 2 * full : 0;
+      for (int x = ua + max(full, 0); x < ub; ++x) {
+        const int left = tiles16 - (8 * x + 2 * warp);
+        if (left <= 0) break;
+        count += min(left, 2);
+      }
     }
-  }
+    Keys<D, DV> kp;
+    Values<D, DV> vp;
+    const long long row = (seq * a.Hk + hk) * a.cap + 16LL * tile0;
+    kp.at(a, row, g, t);
+    vp.at(a, row, g, t);
+    KeyFrag<D, DV> kf[2];
+    ValueFrag<D, DV> vf[2];
+    if (count > 0) { kf[0].load(kp, 0); vf[0].load(vp, 0); }
+    if (count > 1) { kf[1].load(kp, 16); vf[1].load(vp, 16); }
 
-  float o[DV / 16][NT][4], m[NT][2], l[NT][2];
-#pragma unroll
-  for (int i = 0; i < DV / 16; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.f;
-#pragma unroll
-  for (int j = 0; j < NT; ++j) { m[j][0] = m[j][1] = -INFINITY; l[j][0] = l[j][1] = 0.f; }
-
-  const int blocks = (most + kBlock - 1) / kBlock, per = (blocks + a.splits - 1) / a.splits;
-  const int end = min(blocks, (split + 1) * per);
-  for (int blk = split * per + warp; blk < end; blk += kAttnWarps) {
-    const int t0 = blk * kBlock;
-    Frag<D, DV> f[2];
-    float s[2][NT][4];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      if (h == 0 || t0 + 16 < most) f[h].load(a, bh, t0 + 16 * h, g, t);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int th = t0 + 16 * h;
-      if (h == 0 || th < most) scores_of<D, DV, NT>(f[h], q, s[h]);
-      if (th + 16 > least) {
+    auto step = [&](KeyFrag<D, DV>& k, ValueFrag<D, DV>& v, int ahead, int token, bool more) {
+      float s[NT][4];
+      uint32_t p[NT][2];
+      scores_of<D, DV, NT>(k, q, s, un);
+      if (more) k.load(kp, ahead);
+      if (token + 16 > least) {
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (th + g + 8 * (e >> 1) >= vis[j][e & 1]) s[h][j][e] = -INFINITY;
-        f[h].cut(th, most, t);
+          for (int e = 0; e < 4; ++e) {
+            const int r = r0 + 8 * j + 2 * t + (e & 1);
+            const int vis = r < R && a.causal ? max(0, n - a.Lq + 1 + r / G) : most;
+            if (token + g + 8 * (e >> 1) >= vis) s[j][e] = -INFINITY;
+          }
+        v.cut(most - token, t);
       }
+      run.weigh(s, a.scale_log2, p);
+      add_values<D, DV, NT>(v, p, run.o, un);
+      if (more) v.load(vp, ahead);
+    };
+    int token = 16 * tile0;
+    for (int i = 0; i < count; i += 2) {
+      step(kf[0], vf[0], kUnit, token, i + 2 < count);
+      if (i + 1 < count) step(kf[1], vf[1], kUnit + 16, token + 16, i + 3 < count);
+      kp.skip(kUnit);
+      vp.skip(kUnit);
+      token += kUnit;
     }
+
+    // the four warps meet
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      float mx[2];
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        mx[e] = fmaxf(fmaxf(s[0][j][e], s[0][j][e + 2]), fmaxf(s[1][j][e], s[1][j][e + 2]));
+        const int r = 8 * j + 2 * t + e;
+        float l = run.l[j][e];
 #pragma unroll
-        for (int off = 4; off < 32; off <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], off));
-        mx[e] = fmaxf(mx[e] * a.scale_log2, m[j][e]);
-      }
-      const float ref0 = mx[0] == -INFINITY ? 0.f : mx[0], ref1 = mx[1] == -INFINITY ? 0.f : mx[1];
-      if (__any_sync(0xffffffffu, mx[0] != m[j][0] || mx[1] != m[j][1])) {
-        const float c0 = ex2_approx(m[j][0] - ref0), c1 = ex2_approx(m[j][1] - ref1);
-        l[j][0] *= c0;
-        l[j][1] *= c1;
+        for (int off = 4; off < 32; off <<= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+        if (g == 0) {
+          sm[warp][r] = -run.nref[j][e];
+          sl[warp][r] = l;
+        }
 #pragma unroll
         for (int i = 0; i < DV / 16; ++i) {
-          o[i][j][0] *= c0; o[i][j][1] *= c1; o[i][j][2] *= c0; o[i][j][3] *= c1;
+          so[warp][r][channel_of<DV>(i, g, 0)] = run.o[i][j][e];
+          so[warp][r][channel_of<DV>(i, g, 1)] = run.o[i][j][e + 2];
         }
-        m[j][0] = mx[0];
-        m[j][1] = mx[1];
       }
+    __syncthreads();
+    const bool alone = ua == 0 && ub == units;
+    const long long slot = 2LL * blockIdx.x + (first_of_share ? 0 : 1);
+    for (int i = threadIdx.x; i < ROWS * (DV / 2); i += blockDim.x) {
+      const int rr = i / (DV / 2), c = 2 * (i - rr * (DV / 2)), r = r0 + rr;
+      if (r >= R) break;
+      float all = sm[0][rr], sum = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int w = 1; w < kAttnWarps; ++w) all = fmaxf(all, sm[w][rr]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[h][j][e] = ex2_approx(fmaf(s[h][j][e], a.scale_log2, -((e & 1) ? ref1 : ref0)));
-          l[j][e & 1] += s[h][j][e];
-        }
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (h == 1 && t0 + 16 >= most) break;
-      uint32_t p[NT][2];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        p[j][0] = transpose8(pack_bf16x2(s[h][j][0], s[h][j][1]));
-        p[j][1] = transpose8(pack_bf16x2(s[h][j][2], s[h][j][3]));
+      for (int w = 0; w < kAttnWarps; ++w) {
+        const float f = ex2_approx(sm[w][rr] - all);
+        sum += f * sl[w][rr];
+        x += f * so[w][rr][c];
+        y += f * so[w][rr][c + 1];
       }
-      add_values<D, DV, NT>(f[h], p, o);
-    }
-  }
-
-  // the four warps meet
-#pragma unroll
-  for (int j = 0; j < NT; ++j)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-#pragma unroll
-      for (int off = 4; off < 32; off <<= 1) l[j][e] += __shfl_xor_sync(0xffffffffu, l[j][e], off);
-      if (g == 0) {
-        sm[warp][8 * j + 2 * t + e] = m[j][e];
-        sl[warp][8 * j + 2 * t + e] = l[j][e];
+      if (alone) {
+        const long long orow = (seq * a.Lq + r / G) * a.H + hk * G + r % G;   // o is token-major
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;                      // a row that sees nothing gives zeros
+        *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.o) + orow * DV + c) =
+            pack_bf16x2(x * inv, y * inv);
+      } else {
+        *reinterpret_cast<float2*>(a.part_o + (slot * ROWS + rr) * DV + c) = make_float2(x, y);
+        if (c == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * (slot * ROWS + rr)) = make_float2(all, sum);
       }
-    }
-  for (int i = threadIdx.x; i < ROWS * DV; i += blockDim.x) so[i / DV][i % DV] = 0.f;
-  __syncthreads();
-  for (int w = 0; w < kAttnWarps; ++w) {
-    if (warp == w) {
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int r = 8 * j + 2 * t + e;
-          float all = -INFINITY;
-#pragma unroll
-          for (int x = 0; x < kAttnWarps; ++x) all = fmaxf(all, sm[x][r]);
-          const float c = m[j][e] == -INFINITY ? 0.f : ex2_approx(m[j][e] - all);
-#pragma unroll
-          for (int i = 0; i < DV / 16; ++i) {
-            so[r][channel_of<DV>(i, g, 0)] += c * o[i][j][e];
-            so[r][channel_of<DV>(i, g, 1)] += c * o[i][j][e + 2];
-          }
-        }
     }
     __syncthreads();
-  }
-  for (int i = threadIdx.x; i < ROWS * (DV / 2); i += blockDim.x) {
-    const int rr = i / (DV / 2), c = 2 * (i - rr * (DV / 2)), r = r0 + rr;
-    if (r >= R) continue;
-    float all = -INFINITY, sum = 0.f;
-#pragma unroll
-    for (int x = 0; x < kAttnWarps; ++x) all = fmaxf(all, sm[x][rr]);
-#pragma unroll
-    for (int x = 0; x < kAttnWarps; ++x)
-      sum += sm[x][rr] == -INFINITY ? 0.f : sl[x][rr] * ex2_approx(sm[x][rr] - all);
-    const int head = hk * G + r % G, qi = r / G;
-    const long long orow = (b * a.Lq + qi) * a.H + head;         // o is token-major
-    if (a.splits == 1) {
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;            // a row that sees nothing gives zeros
-      *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.o) + orow * DV + c) =
-          pack_bf16x2(so[rr][c] * inv, so[rr][c + 1] * inv);
-    } else {
-      const long long part = orow * a.splits + split;
-      *reinterpret_cast<float2*>(a.part_o + part * DV + c) = make_float2(so[rr][c], so[rr][c + 1]);
-      if (c == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * part) = make_float2(all, sum);
-    }
+    first_of_share = false;
+    seq = seq_next;
   }
 }
 
-// joins the splits of one row: a warp a row
-template <int DV>
-__global__ void __launch_bounds__(128) kv4_join_k(const Kv4AttnArgs a) {
-  const long long row = static_cast<long long>(blockIdx.x) * 4 + threadIdx.x / 32;
-  if (row >= a.B * a.Lq * a.H) return;
-  const int lane = threadIdx.x % 32;
-  const float* ml = a.part_ml + 2 * row * a.splits;
-  const float* po = a.part_o + row * a.splits * DV;
-  float all = -INFINITY;
-  for (int s = lane; s < a.splits; s += 32) all = fmaxf(all, ml[2 * s]);
-  all = warp_max(all);
-  constexpr int N = DV / 32;
-  float acc[N], sum = 0.f;
+// One CTA a row of an item whose units several CTAs of the first kernel shared:
+// its parts, in order, over the four warps, then the warps.
+template <int DV, int NT>
+__global__ void __launch_bounds__(128) kv4_join_k(const Kv4AttnArgs a, int ctas) {
+  constexpr int ROWS = 8 * NT, N = DV / 32;
+  __shared__ float sm[4], sl[4], so[4][DV];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int G = a.H / a.Hk, R = G * a.Lq, tiles = (R + ROWS - 1) / ROWS, per = a.Hk * tiles;
+  const int item = blockIdx.x % per, hk = item / tiles, rr = blockIdx.y, r = (item - hk * tiles) * ROWS + rr;
+  const long long seq = blockIdx.x / per;
+  if (r >= R) return;
+  long long before = 0, total, none;
+  if (a.lengths == nullptr) {
+    total = scan_units(a, per, -1, none, none);
+    before = seq * (total / a.B);
+  } else {
+    total = 0;
+    long long mine = 0;
+    for (long long b = lane; b < a.B; b += 32) {
+      const long long x = kHead + units_of(length_of(a, b));
+      total += x;
+      if (b < seq) mine += x;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      total += __shfl_xor_sync(0xffffffffu, total, o);
+      mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    }
+    total *= per;
+    before = mine * per;
+  }
+  const long long share = (total + ctas - 1) / ctas, units = units_of(length_of(a, seq));
+  const long long u0 = before + item * (kHead + units) + kHead, c0 = u0 / share, c1 = (u0 + units - 1) / share;
+  if (c0 == c1) return;                                // one CTA had it whole and has written it
+  // it is the first item of CTA c0's share where that begins with it (or with its blank units)
+  float acc[N], m = -kUnset, l = 0.f;
 #pragma unroll
   for (int j = 0; j < N; ++j) acc[j] = 0.f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float ms = ml[2 * s];
-    if (ms == -INFINITY) continue;
-    const float c = ex2_approx(ms - all);
-    sum += c * ml[2 * s + 1];
+  for (long long c = c0 + warp; c <= c1; c += 4) {
+    const long long at = (2 * c + (c == c0 && c0 * share < u0 - kHead ? 1 : 0)) * ROWS + rr;
+    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * at);
+    const float to = fmaxf(m, ml.x), keep = ex2_approx(m - to), add = ex2_approx(ml.x - to);
+    m = to;
+    l = l * keep + ml.y * add;
+    const float* po = a.part_o + at * DV + N * lane;
 #pragma unroll
-    for (int j = 0; j < N; ++j) acc[j] += c * po[static_cast<long long>(s) * DV + N * lane + j];
+    for (int j = 0; j < N; ++j) acc[j] = acc[j] * keep + po[j] * add;
+  }
+  if (lane == 0) { sm[warp] = m; sl[warp] = l; }
+#pragma unroll
+  for (int j = 0; j < N; ++j) so[warp][N * lane + j] = acc[j];
+  __syncthreads();
+  if (threadIdx.x >= DV / 2) return;
+  const float all = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+  float sum = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float c = ex2_approx(sm[w] - all);
+    sum += c * sl[w];
+    x += c * so[w][2 * threadIdx.x];
+    y += c * so[w][2 * threadIdx.x + 1];
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.o) + row * DV + N * lane;
-#pragma unroll
-  for (int j = 0; j < N; j += 2) *reinterpret_cast<uint32_t*>(o + j) = pack_bf16x2(acc[j] * inv, acc[j + 1] * inv);
+  const long long orow = (seq * a.Lq + r / G) * a.H + hk * G + r % G;
+  *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.o) + orow * DV + 2 * threadIdx.x) =
+      pack_bf16x2(x * inv, y * inv);
 }
 
-template <int D, int DV>
+int tiles_of(const Kv4AttnArgs& a) { return a.H / a.Hk * a.Lq <= 8 ? 1 : 2; }
+
+template <int D, int DV, int NT>
 int attn_launch(const Kv4AttnArgs& a, cudaStream_t st) {
-  const int R = a.H / a.Hk * a.Lq, NT = kv4_attn_tiles(a);
-  const dim3 grid(a.splits, a.Hk * ((R + 8 * NT - 1) / (8 * NT)), static_cast<unsigned>(a.B));
-  if (grid.y > 65535 || a.B > 65535) return 2;
-  if (NT == 1) kv4_attn_k<D, DV, 1><<<grid, 32 * kAttnWarps, 0, st>>>(a);
-  else kv4_attn_k<D, DV, 2><<<grid, 32 * kAttnWarps, 0, st>>>(a);
+  const long long items = a.B * a.Hk * ((static_cast<long long>(a.H / a.Hk) * a.Lq + 8 * NT - 1) / (8 * NT));
+  if (items > 0x7fffffffLL) return 2;
+  kv4_attn_k<D, DV, NT><<<a.ctas, 32 * kAttnWarps, 0, st>>>(a);
   if (cudaGetLastError() != cudaSuccess) return 3;
-  if (a.splits > 1) {
-    const long long rows = a.B * a.Lq * a.H;
-    kv4_join_k<DV><<<static_cast<unsigned>((rows + 3) / 4), 128, 0, st>>>(a);
-    if (cudaGetLastError() != cudaSuccess) return 3;
-  }
-  return 0;
+  kv4_join_k<DV, NT><<<dim3(static_cast<unsigned>(items), 8 * NT), 128, 0, st>>>(a, a.ctas);
+  return cudaGetLastError() == cudaSuccess ? 0 : 3;
 }
 
 }  // namespace
@@ -542,35 +705,40 @@ int kv4_append(const Kv4AppendArgs& a, int type, cudaStream_t st) {
   return cudaGetLastError() == cudaSuccess ? 0 : 3;
 }
 
-int kv4_read(const Kv4ReadArgs& a, cudaStream_t st) {
+int kv4_read(Kv4ReadArgs a, cudaStream_t st) {
   if (a.D % kGroup || a.Dv % kGroup || a.D < kGroup || a.Dv < kGroup) return 1;
   if (a.B * a.L * a.Hk == 0) return 0;
   const long long most = a.B * a.L * a.Hk * ((a.D > a.Dv ? a.D : a.Dv) / 8), blocks = (most + 255) / 256;
   if (blocks > 0x7fffffffLL) return 2;
+  a.mask = 0x000F000Fu;
+  a.magic = 0x43004300u;
   kv4_read_k<<<dim3(static_cast<unsigned>(blocks), 2), 256, 0, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? 0 : 3;
 }
 
-int kv4_attn_tiles(const Kv4AttnArgs& a) { return a.H / a.Hk * a.Lq <= 8 ? 1 : 2; }
-
-// Splits of the tokens: enough CTAs for three a SM, each warp of a split with
-// one block of 32 tokens at least.
-int kv4_attn_splits(const Kv4AttnArgs& a, long long most_tokens) {
-  const int NT = kv4_attn_tiles(a);
+// CTAs: as many as run at once, or one a unit where there are fewer units.
+// Scratch: two partial tiles a CTA.
+void kv4_attn_plan(Kv4AttnArgs& a, long long most_tokens) {
+  const int NT = tiles_of(a);
   const long long tiles = (static_cast<long long>(a.H / a.Hk) * a.Lq + 8 * NT - 1) / (8 * NT);
-  const long long ctas = a.B * a.Hk * tiles, blocks = (most_tokens + kBlock - 1) / kBlock;
-  long long s = (148 * 3 + ctas - 1) / ctas, most = (blocks + kAttnWarps - 1) / kAttnWarps;
-  if (s > most) s = most;
-  return static_cast<int>(s < 1 ? 1 : s);
+  const long long units = a.B * a.Hk * tiles * (kHead + (most_tokens <= kUnit ? 1 : (most_tokens + kUnit - 1) / kUnit));
+  a.mask = 0x000F000Fu;
+  a.magic = 0x43004300u;
+  const long long most = 148 * (NT == 1 ? 3 : 2);
+  a.ctas = static_cast<int>(units < most ? units : most);
+  a.part_rows = 2LL * a.ctas * 8 * NT;
 }
 
 int kv4_attn(const Kv4AttnArgs& a, cudaStream_t st) {
-  if (a.Hk < 1 || a.H % a.Hk || a.splits < 1 || a.cap % 16) return 1;
+  if (a.Hk < 1 || a.H % a.Hk || a.ctas < 1 || a.cap % 16) return 1;
   if (a.B * a.H * a.Lq == 0) return 0;
-  if (a.D == 64 && a.Dv == 64) return attn_launch<64, 64>(a, st);
-  if (a.D == 64 && a.Dv == 128) return attn_launch<64, 128>(a, st);
-  if (a.D == 128 && a.Dv == 64) return attn_launch<128, 64>(a, st);
-  if (a.D == 128 && a.Dv == 128) return attn_launch<128, 128>(a, st);
+#define VAGUS_KV4_ATTN(D_, DV_) \
+  if (a.D == D_ && a.Dv == DV_) return tiles_of(a) == 1 ? attn_launch<D_, DV_, 1>(a, st) : attn_launch<D_, DV_, 2>(a, st)
+  VAGUS_KV4_ATTN(64, 64);
+  VAGUS_KV4_ATTN(64, 128);
+  VAGUS_KV4_ATTN(128, 64);
+  VAGUS_KV4_ATTN(128, 128);
+#undef VAGUS_KV4_ATTN
   return 1;
 }
 
