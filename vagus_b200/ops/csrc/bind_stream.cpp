@@ -217,10 +217,12 @@ c10::optional<Tensor> kv4_attn(Tensor q, Tensor kc, Tensor kp, Tensor vc, Tensor
   a.o = o.data_ptr();
   Tensor part;
   if (o.numel() > 0) {
-    vagus::kv4_attn_plan(a, a.lengths ? c.cap : length);
-    part = at::empty({a.part_rows * (c.Dv + 2)}, q.options().dtype(at::kFloat));
-    a.part_o = part.data_ptr<float>();
-    a.part_ml = a.part_o + a.part_rows * c.Dv;
+    check(vagus::kv4_attn_plan(a, a.lengths ? c.cap : length), "kv4_attn");
+    if (a.part_rows > 0) {
+      part = at::empty({a.part_rows * (c.Dv + 2)}, q.options().dtype(at::kFloat));
+      a.part_o = part.data_ptr<float>();
+      a.part_ml = a.part_o + a.part_rows * c.Dv;
+    }
     check(vagus::kv4_attn(a, at::cuda::getCurrentCUDAStream().stream()), "kv4_attn");
   }
   return o.transpose(1, 2);

@@ -225,7 +225,7 @@ struct Kv4ReadArgs {
   void *k, *v;                                  // (B, Hk, L, D | Dv) bf16 dense
   const void* start; int start_i64; long long offset;
   long long B, L, cap; int Hk, D, Dv;
-  unsigned mask, magic;                         // set by kv4_read
+  unsigned magic;                               // set by kv4_read
   int* err;
 };
 int kv4_read(Kv4ReadArgs a, cudaStream_t st);
@@ -238,11 +238,11 @@ struct Kv4AttnArgs {
   const void* lengths; int len_i64; long long length;       // tokens held per sequence, or null: length
   long long B, cap; int H, Hk, Lq, D, Dv, causal;
   float scale_log2;                             // softmax scale times log2(e)
-  int ctas; long long part_rows; unsigned mask, magic;      // set by kv4_attn_plan
+  int ctas, cluster; long long part_rows; unsigned magic;   // set by kv4_attn_plan
   float *part_o, *part_ml;                      // scratch (part_rows, Dv | 2) fp32
   int* err;
 };
-void kv4_attn_plan(Kv4AttnArgs& a, long long most_tokens);
+int kv4_attn_plan(Kv4AttnArgs& a, long long most_tokens);
 int kv4_attn(const Kv4AttnArgs& a, cudaStream_t st);
 
 // verify.cu: verification of drafted tokens (see verify.cu).  type: 0 fp32, 1 fp16, 2 bf16.

@@ -126,17 +126,13 @@ __device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t 
   asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
   return d;
 }
-// The two constants of unpacking, from the kernel's arguments: the logic operation
-// takes one immediate at most, and with both known to the compiler each unpacking
-// costs two of them.
-struct Unpack {
-  uint32_t mask, magic;          // 0x000F000F, 0x43004300
-};
-// nibbles i and i + 4 of w (i = 0 .. 3) as the pair of values they stand for
+// Nibbles i and i + 4 of w (i = 0 .. 3) as the pair of values they stand for.  magic is 0x43004300, from the
+// kernel's arguments: the logic operation takes one immediate at most, and with both constants known to the
+// compiler each unpacking cost two operations (attention over 2 x 131067 tokens 90 us instead of 76).
 template <int I>
-__device__ __forceinline__ uint32_t pair_of(uint32_t w, uint32_t ss, uint32_t bb, const Unpack& c) {
+__device__ __forceinline__ uint32_t pair_of(uint32_t w, uint32_t ss, uint32_t bb, uint32_t magic) {
   uint32_t x;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(x) : "r"(w >> (4 * I)), "r"(c.mask), "r"(c.magic));   // (w & mask) | magic
+  asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;" : "=r"(x) : "r"(w >> (4 * I)), "r"(magic));   // (w & mask) | magic
   return fma_bf16x2(x, ss, bb);
 }
 __device__ __forceinline__ uint32_t low2(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x5410); }
@@ -163,7 +159,7 @@ __global__ void __launch_bounds__(256) kv4_read_k(const Kv4ReadArgs a) {
   const long long at = bh * a.cap + t;
   const uint32_t w = codes[at * per + cw], p = params[at * (D / kGroup) + cw / 4];
   const uint32_t ss = low2(p, p), bb = high2(p, p);
-  const Unpack un{a.mask, a.magic};
+  const uint32_t un = a.magic;
   const uint32_t p0 = pair_of<0>(w, ss, bb, un), p1 = pair_of<1>(w, ss, bb, un), p2 = pair_of<2>(w, ss, bb, un),
                  p3 = pair_of<3>(w, ss, bb, un);
   out[i] = make_uint4(low2(p0, p1), low2(p2, p3), high2(p0, p1), high2(p2, p3));
@@ -192,16 +188,29 @@ __global__ void __launch_bounds__(256) kv4_read_k(const Kv4ReadArgs a) {
 // of the output's own rounding); scores, sums and accumulators are fp32.
 //
 // Work.  An item is a row tile of one KV head of one sequence; its tokens are cut
-// into units of 128 (each of a CTA's four warps takes 32 of them).  All items'
-// units, laid end to end with two blank ones ahead of each item (what starting and
-// ending it costs), are dealt to the CTAs in equal contiguous shares, so ragged
-// batches and few long sequences fill the GPU alike.  A CTA writes the
-// items it has whole; of the first and last item of its share it may have a part,
-// which it leaves in slot 0 or 1 of its scratch, and the join kernel adds the
-// parts of an item in order.
+// into units of 128 (each of a CTA's four warps takes 32 of them).  There are two ways
+// to deal them out, and kv4_attn_plan picks the one that should end first:
+//
+// - by clusters: equal lengths known to the host, an item to a cluster of up to 8 CTAs
+//   whose parts meet in distributed shared memory.  One launch.
+// - flat: all items' units, laid end to end with two blank ones ahead of each item (what
+//   starting and ending it costs), go to the CTAs in equal contiguous shares, so ragged
+//   batches and few long sequences fill the GPU alike.  A CTA writes the items it has
+//   whole; of the first and last item of its share it may have a part, which it leaves in
+//   slot 0 or 1 of its scratch, and a second kernel adds the parts of an item in order.
+//
+// What bounds it: the unpacking.  Of 16 tokens x 128 channels of K and V a warp does 64
+// shift / mask-or / fma triples, 16 products and 12 permutes, and the logic operations
+// issue at half rate next to fmas and products that share ports with them; measured with
+// its loads served by L2 it takes 73 us for what takes 74 from HBM and whose bytes alone
+// take 52 (2 x 131067 tokens, 8 KV heads of 128: 4.5 TB/s).  A ring of bulk copies into
+// shared memory with 8, 12 or 16 warps an SM, and scores formed one block ahead, all
+// measured the same within 4 percent; loads two tiles ahead into registers are the
+// simplest of them.
 
 constexpr int kAttnWarps = 4;
 constexpr int kUnit = 32 * kAttnWarps;      // tokens
+constexpr int kMaxCluster = 8;
 constexpr int kHead = 2;                    // what starting and ending an item costs, in units
 constexpr float kUnset = 1e30f;             // minus the softmax reference before the first score
 constexpr float kLazy = 8.f;                // raise the reference when a score exceeds it by so many powers of 2
@@ -285,7 +294,7 @@ struct Query {
 };
 
 template <int D, int DV, int NT>
-__device__ __forceinline__ void scores_of(const KeyFrag<D, DV>& f, const Query<D, NT>& q, float (&s)[NT][4], const Unpack& un) {
+__device__ __forceinline__ void scores_of(const KeyFrag<D, DV>& f, const Query<D, NT>& q, float (&s)[NT][4], uint32_t un) {
 #pragma unroll
   for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
   const uint32_t s0 = low2(f.p[0], f.p[0]), b0 = high2(f.p[0], f.p[0]);
@@ -307,7 +316,7 @@ __device__ __forceinline__ void scores_of(const KeyFrag<D, DV>& f, const Query<D
 
 template <int D, int DV, int NT>
 __device__ __forceinline__ void add_values(const ValueFrag<D, DV>& f, const uint32_t (&p)[NT][2],
-                                           float (&o)[DV / 16][NT][4], const Unpack& un) {
+                                           float (&o)[DV / 16][NT][4], uint32_t un) {
   constexpr int W = DV / 64;
   const uint32_t sl = low2(f.p[0], f.p[1]), bl = high2(f.p[0], f.p[1]);
   const uint32_t sh = low2(f.p[2], f.p[3]), bh = high2(f.p[2], f.p[3]);
@@ -414,22 +423,22 @@ __device__ __forceinline__ int length_of(const Kv4AttnArgs& a, long long b) {
 __device__ __forceinline__ int units_of(int n) { return n <= kUnit ? 1 : (n + kUnit - 1) / kUnit; }
 
 // One warp: units (blank ones included) of all sequences (times `per` items each), and with
-// `flat` >= 0 the sequence that holds unit `flat` and the units before it.
-__device__ long long scan_units(const Kv4AttnArgs& a, int per, long long flat, long long& seq, long long& before) {
+// `flat` >= 0 the sequence that holds unit `flat` and the units before it.  The host has
+// checked that the units fit 31 bits.
+__device__ int scan_units(const Kv4AttnArgs& a, int per, int flat, int& seq, int& before) {
   const int lane = threadIdx.x % 32;
   if (a.lengths == nullptr) {
-    const long long u = static_cast<long long>(kHead + units_of(static_cast<int>(a.length))) * per;
+    const int u = (kHead + units_of(static_cast<int>(a.length))) * per;
     if (flat >= 0) { seq = flat / u; before = seq * u; }
-    return u * a.B;
+    return u * static_cast<int>(a.B);
   }
-  long long run = 0;
-  for (long long b0 = 0; b0 < a.B; b0 += 32) {
-    const long long b = b0 + lane;
-    const long long u = b < a.B ? static_cast<long long>(kHead + units_of(length_of(a, b))) * per : 0;
-    long long in = u;
+  int run = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 32) {
+    const int b = b0 + lane, u = b < a.B ? (kHead + units_of(length_of(a, b))) * per : 0;
+    int in = u;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long up = __shfl_up_sync(0xffffffffu, in, o);
+      const int up = __shfl_up_sync(0xffffffffu, in, o);
       if (lane >= o) in += up;
     }
     const unsigned hit = __ballot_sync(0xffffffffu, flat >= 0 && run + in > flat);
@@ -444,205 +453,218 @@ __device__ long long scan_units(const Kv4AttnArgs& a, int per, long long flat, l
   return run;
 }
 
-template <int D, int DV, int NT>
-__global__ void __launch_bounds__(32 * kAttnWarps, NT == 1 ? 3 : 2) kv4_attn_k(const Kv4AttnArgs a) {
-  constexpr int ROWS = 8 * NT;
-  __shared__ float sm[kAttnWarps][ROWS], sl[kAttnWarps][ROWS];
-  __shared__ float so[kAttnWarps][ROWS][DV + 4];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane >> 2, t = lane & 3;
-  const int G = a.H / a.Hk, R = G * a.Lq, tiles = (R + ROWS - 1) / ROWS, per = a.Hk * tiles;
+// What the four warps of a CTA have of one part of an item.
+template <int DV, int NT>
+struct Part {
+  static constexpr int ROWS = 8 * NT;
+  float m[kAttnWarps][ROWS], l[kAttnWarps][ROWS];       // softmax reference and sum
+  float o[kAttnWarps][ROWS][DV + 4];
+  // row rr, channels c and c + 1, over the warps
+  __device__ __forceinline__ void join(int rr, int c, float& top, float& sum, float& x, float& y) const {
+    top = m[0][rr];
+    sum = x = y = 0.f;
+#pragma unroll
+    for (int w = 1; w < kAttnWarps; ++w) top = fmaxf(top, m[w][rr]);
+#pragma unroll
+    for (int w = 0; w < kAttnWarps; ++w) {
+      const float f = ex2_approx(m[w][rr] - top);
+      sum += f * l[w][rr];
+      x += f * o[w][rr][c];
+      y += f * o[w][rr][c + 1];
+    }
+  }
+};
 
-  long long seq = 0, before = 0;
-  const long long total = scan_units(a, per, -1, seq, before);
-  const long long share = (total + gridDim.x - 1) / gridDim.x;
-  long long u = blockIdx.x * share;
-  const long long end = min(total, u + share);
+// Units [ua, ub) of an item (sequence seq of n tokens) into part; ends with a barrier.
+template <int D, int DV, int NT>
+__device__ __forceinline__ void attend(const Kv4AttnArgs& a, int seq, int n, int hk, int r0, int ua, int ub,
+                                       Part<DV, NT>& part) {
+  constexpr int ROWS = 8 * NT;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane >> 2, t = lane & 3;
+  const int G = a.H / a.Hk, R = G * a.Lq;
+  const uint32_t un = a.magic;
+  // a row sees the first `vis` tokens; the tile between `least` and `most`
+  const int first = r0 / G, last = (min(r0 + ROWS, R) - 1) / G;
+  const int least = a.causal ? max(0, n - a.Lq + 1 + first) : n;
+  const int most = a.causal ? max(0, n - a.Lq + 1 + last) : n;
+
+  // this warp's tiles of 16 tokens: two neighbouring ones of every unit, up to `most`
+  const int tile0 = 8 * ua + 2 * warp, tiles16 = min((most + 15) / 16, 8 * ub);
+  const int left = tiles16 - tile0, count = left > 0 ? left / 8 * 2 + min(left % 8, 2) : 0;
+  Keys<D, DV> kp;
+  Values<D, DV> vp;
+  const long long row = (static_cast<long long>(seq) * a.Hk + hk) * a.cap + 16LL * tile0;
+  kp.at(a, row, g, t);
+  vp.at(a, row, g, t);
+  KeyFrag<D, DV> kf[2];
+  ValueFrag<D, DV> vf[2];
+  if (count > 0) { kf[0].load(kp, 0); vf[0].load(vp, 0); }
+  if (count > 1) { kf[1].load(kp, 16); vf[1].load(vp, 16); }
+
+  Query<D, NT> q;
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int r = r0 + 8 * j + g;
+    const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(a.q) + seq * a.sq_b + (hk * G + r % G) * a.sq_h +
+                               static_cast<long long>(r / G) * a.sq_l;
+#pragma unroll
+    for (int w = 0; w < D / 32; ++w) {
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (r < R) x = *reinterpret_cast<const uint4*>(src + 8 * (t * (D / 32) + w));
+      q.b[j][2 * w][0] = low2(x.x, x.z);          // channels (0, 4)
+      q.b[j][2 * w][1] = high2(x.x, x.z);         // (1, 5)
+      q.b[j][2 * w + 1][0] = low2(x.y, x.w);      // (2, 6)
+      q.b[j][2 * w + 1][1] = high2(x.y, x.w);     // (3, 7)
+    }
+  }
+
+  Running<D, DV, NT> run;
+  run.clear();
+  // a tile's own registers are loaded again, for the tile two on, as soon as they are used
+  auto step = [&](KeyFrag<D, DV>& k, ValueFrag<D, DV>& v, int ahead, int token, bool more) {
+    float s[NT][4];
+    uint32_t p[NT][2];
+    scores_of<D, DV, NT>(k, q, s, un);
+    if (more) k.load(kp, ahead);
+    if (token + 16 > least) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = r0 + 8 * j + 2 * t + (e & 1);
+          const int vis = r < R && a.causal ? max(0, n - a.Lq + 1 + r / G) : most;
+          if (token + g + 8 * (e >> 1) >= vis) s[j][e] = -INFINITY;
+        }
+      v.cut(most - token, t);
+    }
+    run.weigh(s, a.scale_log2, p);
+    add_values<D, DV, NT>(v, p, run.o, un);
+    if (more) v.load(vp, ahead);
+  };
+  for (int i = 0, token = 16 * tile0; i < count; i += 2, token += kUnit) {
+    step(kf[0], vf[0], kUnit, token, i + 2 < count);
+    if (i + 1 < count) step(kf[1], vf[1], kUnit + 16, token + 16, i + 3 < count);
+    kp.skip(kUnit);
+    vp.skip(kUnit);
+  }
+
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = 8 * j + 2 * t + e;
+      float l = run.l[j][e];
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+      if (g == 0) {
+        part.m[warp][r] = -run.nref[j][e];
+        part.l[warp][r] = l;
+      }
+#pragma unroll
+      for (int i = 0; i < DV / 16; ++i) {
+        part.o[warp][r][channel_of<DV>(i, g, 0)] = run.o[i][j][e];
+        part.o[warp][r][channel_of<DV>(i, g, 1)] = run.o[i][j][e + 2];
+      }
+    }
+  __syncthreads();
+}
+
+// row r of KV head hk, channels c and c + 1; o is token-major.  A row that sees nothing gives zeros.
+template <int DV>
+__device__ __forceinline__ void store_row(const Kv4AttnArgs& a, int seq, int hk, int r, int c, float sum, float x, float y) {
+  const int G = a.H / a.Hk;
+  const long long row = (static_cast<long long>(seq) * a.Lq + r / G) * a.H + hk * G + r % G;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.o) + row * DV + c) = pack_bf16x2(x * inv, y * inv);
+}
+
+constexpr int ctas_per_sm(int NT) { return NT == 1 ? 3 : 2; }
+
+template <int D, int DV, int NT>
+__global__ void __launch_bounds__(32 * kAttnWarps, ctas_per_sm(NT)) kv4_attn_k(const Kv4AttnArgs a) {
+  constexpr int ROWS = 8 * NT;
+  __shared__ Part<DV, NT> part;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int R = a.H / a.Hk * a.Lq, tiles = (R + ROWS - 1) / ROWS, per = a.Hk * tiles;
+  int seq = 0, before = 0;
+  const int total = scan_units(a, per, -1, seq, before);
+  const int share = (total + gridDim.x - 1) / gridDim.x;
+  int u = min(total, static_cast<int>(blockIdx.x) * share);
+  const int end = min(total, u + share);
   if (u >= end) return;
   scan_units(a, per, u, seq, before);
   bool first_of_share = true;
-  const Unpack un{a.mask, a.magic};
 
-  long long seq_next = seq;
   while (u < end) {
     // the item that holds unit u, and the part of it that is this CTA's
     const int n = length_of(a, seq), units = units_of(n);
-    const int item = static_cast<int>((u - before) / (kHead + units));
-    const long long item0 = before + static_cast<long long>(item) * (kHead + units) + kHead;
-    const int ua = static_cast<int>(max(0LL, u - item0)), ub = static_cast<int>(min(end - item0, static_cast<long long>(units)));
-    u = item0 + ub;
-    if (item + 1 == per && ub == units) {
-      before = u;
-      ++seq_next;
-    }
+    const int item = (u - before) / (kHead + units), item0 = before + item * (kHead + units) + kHead;
+    const int ua = max(0, u - item0), ub = min(end - item0, units);
     if (ub <= 0) break;                       // only blank units of it: the next CTA starts it
     const int hk = item / tiles, r0 = (item - hk * tiles) * ROWS;
-    // a row sees the first `vis` tokens; the tile between `least` and `most`
-    const int first = r0 / G, last = (min(r0 + ROWS, R) - 1) / G;
-    const int least = a.causal ? max(0, n - a.Lq + 1 + first) : n;
-    const int most = a.causal ? max(0, n - a.Lq + 1 + last) : n;
+    attend<D, DV, NT>(a, seq, n, hk, r0, ua, ub, part);
 
-    Query<D, NT> q;
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const int r = r0 + 8 * j + g;
-      const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(a.q) + seq * a.sq_b +
-                                 (hk * G + r % G) * a.sq_h + static_cast<long long>(r / G) * a.sq_l;
-#pragma unroll
-      for (int w = 0; w < D / 32; ++w) {
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (r < R) x = *reinterpret_cast<const uint4*>(src + 8 * (t * (D / 32) + w));
-        q.b[j][2 * w][0] = low2(x.x, x.z);          // channels (0, 4)
-        q.b[j][2 * w][1] = high2(x.x, x.z);         // (1, 5)
-        q.b[j][2 * w + 1][0] = low2(x.y, x.w);      // (2, 6)
-        q.b[j][2 * w + 1][1] = high2(x.y, x.w);     // (3, 7)
-      }
-    }
-
-    Running<D, DV, NT> run;
-    run.clear();
-    // this warp's tiles of 16 tokens: two neighbouring ones of every unit, up to `most`
-    const int tile0 = 8 * ua + 2 * warp, tiles16 = (most + 15) / 16;
-    const int whole = (tiles16 - 2 * warp) / 8;                              // units with both tiles
-    int count = 0;
-    if (tiles16 > tile0) {
-      const int full = min(ub, max(0, whole)) - ua;
-      count = full > 0 ? 2 * full : 0;
-      for (int x = ua + max(full, 0); x < ub; ++x) {
-        const int left = tiles16 - (8 * x + 2 * warp);
-        if (left <= 0) break;
-        count += min(left, 2);
-      }
-    }
-    Keys<D, DV> kp;
-    Values<D, DV> vp;
-    const long long row = (seq * a.Hk + hk) * a.cap + 16LL * tile0;
-    kp.at(a, row, g, t);
-    vp.at(a, row, g, t);
-    KeyFrag<D, DV> kf[2];
-    ValueFrag<D, DV> vf[2];
-    if (count > 0) { kf[0].load(kp, 0); vf[0].load(vp, 0); }
-    if (count > 1) { kf[1].load(kp, 16); vf[1].load(vp, 16); }
-
-    auto step = [&](KeyFrag<D, DV>& k, ValueFrag<D, DV>& v, int ahead, int token, bool more) {
-      float s[NT][4];
-      uint32_t p[NT][2];
-      scores_of<D, DV, NT>(k, q, s, un);
-      if (more) k.load(kp, ahead);
-      if (token + 16 > least) {
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int r = r0 + 8 * j + 2 * t + (e & 1);
-            const int vis = r < R && a.causal ? max(0, n - a.Lq + 1 + r / G) : most;
-            if (token + g + 8 * (e >> 1) >= vis) s[j][e] = -INFINITY;
-          }
-        v.cut(most - token, t);
-      }
-      run.weigh(s, a.scale_log2, p);
-      add_values<D, DV, NT>(v, p, run.o, un);
-      if (more) v.load(vp, ahead);
-    };
-    int token = 16 * tile0;
-    for (int i = 0; i < count; i += 2) {
-      step(kf[0], vf[0], kUnit, token, i + 2 < count);
-      if (i + 1 < count) step(kf[1], vf[1], kUnit + 16, token + 16, i + 3 < count);
-      kp.skip(kUnit);
-      vp.skip(kUnit);
-      token += kUnit;
-    }
-
-    // the four warps meet
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int r = 8 * j + 2 * t + e;
-        float l = run.l[j][e];
-#pragma unroll
-        for (int off = 4; off < 32; off <<= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
-        if (g == 0) {
-          sm[warp][r] = -run.nref[j][e];
-          sl[warp][r] = l;
-        }
-#pragma unroll
-        for (int i = 0; i < DV / 16; ++i) {
-          so[warp][r][channel_of<DV>(i, g, 0)] = run.o[i][j][e];
-          so[warp][r][channel_of<DV>(i, g, 1)] = run.o[i][j][e + 2];
-        }
-      }
-    __syncthreads();
     const bool alone = ua == 0 && ub == units;
     const long long slot = 2LL * blockIdx.x + (first_of_share ? 0 : 1);
     for (int i = threadIdx.x; i < ROWS * (DV / 2); i += blockDim.x) {
-      const int rr = i / (DV / 2), c = 2 * (i - rr * (DV / 2)), r = r0 + rr;
-      if (r >= R) break;
-      float all = sm[0][rr], sum = 0.f, x = 0.f, y = 0.f;
-#pragma unroll
-      for (int w = 1; w < kAttnWarps; ++w) all = fmaxf(all, sm[w][rr]);
-#pragma unroll
-      for (int w = 0; w < kAttnWarps; ++w) {
-        const float f = ex2_approx(sm[w][rr] - all);
-        sum += f * sl[w][rr];
-        x += f * so[w][rr][c];
-        y += f * so[w][rr][c + 1];
-      }
+      const int rr = i / (DV / 2), c = 2 * (i - rr * (DV / 2));
+      if (r0 + rr >= R) break;
+      float top, sum, x, y;
+      part.join(rr, c, top, sum, x, y);
       if (alone) {
-        const long long orow = (seq * a.Lq + r / G) * a.H + hk * G + r % G;   // o is token-major
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;                      // a row that sees nothing gives zeros
-        *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.o) + orow * DV + c) =
-            pack_bf16x2(x * inv, y * inv);
+        store_row<DV>(a, seq, hk, r0 + rr, c, sum, x, y);
       } else {
         *reinterpret_cast<float2*>(a.part_o + (slot * ROWS + rr) * DV + c) = make_float2(x, y);
-        if (c == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * (slot * ROWS + rr)) = make_float2(all, sum);
+        if (c == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * (slot * ROWS + rr)) = make_float2(top, sum);
       }
     }
     __syncthreads();
+    u = item0 + ub;
     first_of_share = false;
-    seq = seq_next;
+    if (item + 1 == per && ub == units) {
+      before = u;
+      ++seq;
+    }
   }
 }
 
 // One CTA a row of an item whose units several CTAs of the first kernel shared:
 // its parts, in order, over the four warps, then the warps.
 template <int DV, int NT>
-__global__ void __launch_bounds__(128) kv4_join_k(const Kv4AttnArgs a, int ctas) {
+__global__ void __launch_bounds__(128) kv4_join_k(const Kv4AttnArgs a) {
   constexpr int ROWS = 8 * NT, N = DV / 32;
   __shared__ float sm[4], sl[4], so[4][DV];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int G = a.H / a.Hk, R = G * a.Lq, tiles = (R + ROWS - 1) / ROWS, per = a.Hk * tiles;
+  const int R = a.H / a.Hk * a.Lq, tiles = (R + ROWS - 1) / ROWS, per = a.Hk * tiles;
   const int item = blockIdx.x % per, hk = item / tiles, rr = blockIdx.y, r = (item - hk * tiles) * ROWS + rr;
-  const long long seq = blockIdx.x / per;
-  if (r >= R) return;
-  long long before = 0, total, none;
+  const int seq = blockIdx.x / per;
+  int before = 0, total, none;
   if (a.lengths == nullptr) {
     total = scan_units(a, per, -1, none, none);
-    before = seq * (total / a.B);
+    before = seq * (total / static_cast<int>(a.B));
   } else {
     total = 0;
-    long long mine = 0;
-    for (long long b = lane; b < a.B; b += 32) {
-      const long long x = kHead + units_of(length_of(a, b));
+    for (int b = lane; b < a.B; b += 32) {
+      const int x = (kHead + units_of(length_of(a, b))) * per;
       total += x;
-      if (b < seq) mine += x;
+      if (b < seq) before += x;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       total += __shfl_xor_sync(0xffffffffu, total, o);
-      mine += __shfl_xor_sync(0xffffffffu, mine, o);
+      before += __shfl_xor_sync(0xffffffffu, before, o);
     }
-    total *= per;
-    before = mine * per;
   }
-  const long long share = (total + ctas - 1) / ctas, units = units_of(length_of(a, seq));
-  const long long u0 = before + item * (kHead + units) + kHead, c0 = u0 / share, c1 = (u0 + units - 1) / share;
-  if (c0 == c1) return;                                // one CTA had it whole and has written it
-  // it is the first item of CTA c0's share where that begins with it (or with its blank units)
+  const int share = (total + a.ctas - 1) / a.ctas, units = units_of(length_of(a, seq));
+  const int u0 = before + item * (kHead + units) + kHead, c0 = u0 / share, c1 = (u0 + units - 1) / share;
+  asm volatile("griddepcontrol.wait;" ::: "memory");   // the first kernel is done and its writes are here
+  if (r >= R || c0 == c1) return;                      // one CTA had it whole and has written it
   float acc[N], m = -kUnset, l = 0.f;
 #pragma unroll
   for (int j = 0; j < N; ++j) acc[j] = 0.f;
-  for (long long c = c0 + warp; c <= c1; c += 4) {
-    const long long at = (2 * c + (c == c0 && c0 * share < u0 - kHead ? 1 : 0)) * ROWS + rr;
+  for (int c = c0 + warp; c <= c1; c += 4) {
+    // it is the first item of CTA c0's share where that begins with it (or with its blank units)
+    const long long at = (2LL * c + (c == c0 && c0 * share < u0 - kHead ? 1 : 0)) * ROWS + rr;
     const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * at);
     const float to = fmaxf(m, ml.x), keep = ex2_approx(m - to), add = ex2_approx(ml.x - to);
     m = to;
@@ -656,31 +678,105 @@ __global__ void __launch_bounds__(128) kv4_join_k(const Kv4AttnArgs a, int ctas)
   for (int j = 0; j < N; ++j) so[warp][N * lane + j] = acc[j];
   __syncthreads();
   if (threadIdx.x >= DV / 2) return;
-  const float all = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+  const float top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
   float sum = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    const float c = ex2_approx(sm[w] - all);
+    const float c = ex2_approx(sm[w] - top);
     sum += c * sl[w];
     x += c * so[w][2 * threadIdx.x];
     y += c * so[w][2 * threadIdx.x + 1];
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  const long long orow = (seq * a.Lq + r / G) * a.H + hk * G + r % G;
-  *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.o) + orow * DV + 2 * threadIdx.x) =
-      pack_bf16x2(x * inv, y * inv);
+  store_row<DV>(a, seq, hk, r, 2 * threadIdx.x, sum, x, y);
+}
+
+__device__ __forceinline__ float ld_cluster_f32(const float* p, int rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
+  return v;
+}
+
+// An item a cluster: CTA `rank` of `a.cluster` has an equal share of its units.
+template <int D, int DV, int NT>
+__global__ void __launch_bounds__(32 * kAttnWarps, ctas_per_sm(NT)) kv4_attn_cluster_k(const Kv4AttnArgs a) {
+  constexpr int ROWS = 8 * NT;
+  __shared__ Part<DV, NT> part;
+  __shared__ float top_of[ROWS], sum_of[ROWS];
+  const int R = a.H / a.Hk * a.Lq, tiles = (R + ROWS - 1) / ROWS, per = a.Hk * tiles, C = a.cluster;
+  const int flat = blockIdx.x / C, rank = blockIdx.x - flat * C, seq = flat / per, item = flat - seq * per;
+  const int hk = item / tiles, r0 = (item - hk * tiles) * ROWS;
+  const int n = static_cast<int>(a.length), units = units_of(n), share = (units + C - 1) / C;
+  attend<D, DV, NT>(a, seq, n, hk, r0, min(units, rank * share), min(units, (rank + 1) * share), part);
+
+  const int rows = min(ROWS, R - r0);
+  for (int i = threadIdx.x; i < rows * (DV / 2); i += blockDim.x) {
+    const int rr = i / (DV / 2), c = 2 * (i - rr * (DV / 2));
+    float top, sum, x, y;
+    part.join(rr, c, top, sum, x, y);
+    if (C == 1) {
+      store_row<DV>(a, seq, hk, r0 + rr, c, sum, x, y);
+    } else {                                  // this thread alone reads these places of the warps' parts
+      part.o[0][rr][c] = x;
+      part.o[0][rr][c + 1] = y;
+      if (c == 0) {
+        top_of[rr] = top;
+        sum_of[rr] = sum;
+      }
+    }
+  }
+  if (C == 1) return;
+  cluster_sync();
+  for (int i = rank * blockDim.x + threadIdx.x; i < rows * (DV / 2); i += C * blockDim.x) {
+    const int rr = i / (DV / 2), c = 2 * (i - rr * (DV / 2));
+    float top = -kUnset, sum = 0.f, x = 0.f, y = 0.f, tops[kMaxCluster];
+#pragma unroll
+    for (int k = 0; k < kMaxCluster; ++k) {
+      tops[k] = k < C ? ld_cluster_f32(&top_of[rr], k) : -kUnset;
+      top = fmaxf(top, tops[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < kMaxCluster; ++k) {
+      if (k >= C) break;
+      const float f = ex2_approx(tops[k] - top);
+      sum += f * ld_cluster_f32(&sum_of[rr], k);
+      x += f * ld_cluster_f32(&part.o[0][rr][c], k);
+      y += f * ld_cluster_f32(&part.o[0][rr][c + 1], k);
+    }
+    store_row<DV>(a, seq, hk, r0 + rr, c, sum, x, y);
+  }
+  cluster_sync();                              // nobody leaves while it is read
 }
 
 int tiles_of(const Kv4AttnArgs& a) { return a.H / a.Hk * a.Lq <= 8 ? 1 : 2; }
 
+template <typename... Args>
+int launch_with(void (*kernel)(Args...), dim3 grid, int threads, cudaStream_t st, cudaLaunchAttribute attr, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? 0 : 3;
+}
+
 template <int D, int DV, int NT>
 int attn_launch(const Kv4AttnArgs& a, cudaStream_t st) {
-  const long long items = a.B * a.Hk * ((static_cast<long long>(a.H / a.Hk) * a.Lq + 8 * NT - 1) / (8 * NT));
-  if (items > 0x7fffffffLL) return 2;
+  const int R = a.H / a.Hk * a.Lq;
+  const unsigned items = static_cast<unsigned>(a.B * a.Hk * ((R + 8 * NT - 1) / (8 * NT)));
+  cudaLaunchAttribute attr = {};
+  if (a.cluster > 0) {
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = a.cluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    return launch_with(kv4_attn_cluster_k<D, DV, NT>, dim3(items * a.cluster), 32 * kAttnWarps, st, attr, a);
+  }
   kv4_attn_k<D, DV, NT><<<a.ctas, 32 * kAttnWarps, 0, st>>>(a);
   if (cudaGetLastError() != cudaSuccess) return 3;
-  kv4_join_k<DV, NT><<<dim3(static_cast<unsigned>(items), 8 * NT), 128, 0, st>>>(a, a.ctas);
-  return cudaGetLastError() == cudaSuccess ? 0 : 3;
+  // launched while the first kernel runs; it waits for that one's writes itself
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  return launch_with(kv4_join_k<DV, NT>, dim3(items, R < 8 * NT ? R : 8 * NT), 128, st, attr, a);
 }
 
 }  // namespace
@@ -710,27 +806,38 @@ int kv4_read(Kv4ReadArgs a, cudaStream_t st) {
   if (a.B * a.L * a.Hk == 0) return 0;
   const long long most = a.B * a.L * a.Hk * ((a.D > a.Dv ? a.D : a.Dv) / 8), blocks = (most + 255) / 256;
   if (blocks > 0x7fffffffLL) return 2;
-  a.mask = 0x000F000Fu;
   a.magic = 0x43004300u;
   kv4_read_k<<<dim3(static_cast<unsigned>(blocks), 2), 256, 0, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? 0 : 3;
 }
 
-// CTAs: as many as run at once, or one a unit where there are fewer units.
-// Scratch: two partial tiles a CTA.
-void kv4_attn_plan(Kv4AttnArgs& a, long long most_tokens) {
+// How the units are dealt out (see above).  A way's length is the units of its longest CTA; the flat one's
+// second kernel costs as much as some five units more (3 us against 0.6 to 0.7 us a unit).
+int kv4_attn_plan(Kv4AttnArgs& a, long long most_tokens) {
   const int NT = tiles_of(a);
   const long long tiles = (static_cast<long long>(a.H / a.Hk) * a.Lq + 8 * NT - 1) / (8 * NT);
-  const long long units = a.B * a.Hk * tiles * (kHead + (most_tokens <= kUnit ? 1 : (most_tokens + kUnit - 1) / kUnit));
-  a.mask = 0x000F000Fu;
+  const long long items = a.B * a.Hk * tiles, per_item = most_tokens <= kUnit ? 1 : (most_tokens + kUnit - 1) / kUnit;
+  const long long units = items * (kHead + per_item), slots = 148LL * ctas_per_sm(NT);
+  if (units > 0x3fffffffLL || items > 0x0fffffffLL) return 2;
   a.magic = 0x43004300u;
-  const long long most = 148 * (NT == 1 ? 3 : 2);
-  a.ctas = static_cast<int>(units < most ? units : most);
+  a.ctas = static_cast<int>(units < slots ? units : slots);
   a.part_rows = 2LL * a.ctas * 8 * NT;
+  a.cluster = 0;
+  if (a.lengths == nullptr && items <= slots) {
+    long long c = slots / items;
+    if (c > kMaxCluster) c = kMaxCluster;
+    if (c > per_item) c = per_item;
+    const long long by_cluster = (per_item + c - 1) / c, by_flat = (units + slots - 1) / slots + 5;
+    if (by_cluster <= by_flat) {
+      a.cluster = static_cast<int>(c);
+      a.part_rows = 0;
+    }
+  }
+  return 0;
 }
 
 int kv4_attn(const Kv4AttnArgs& a, cudaStream_t st) {
-  if (a.Hk < 1 || a.H % a.Hk || a.ctas < 1 || a.cap % 16) return 1;
+  if (a.Hk < 1 || a.H % a.Hk || (a.cluster < 1 && a.ctas < 1) || a.cap % 16) return 1;
   if (a.B * a.H * a.Lq == 0) return 0;
 #define VAGUS_KV4_ATTN(D_, DV_) \
   if (a.D == D_ && a.Dv == DV_) return tiles_of(a) == 1 ? attn_launch<D_, DV_, 1>(a, st) : attn_launch<D_, DV_, 2>(a, st)
