@@ -547,7 +547,8 @@ attn_fwd_tc(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUte
       // PV_{j-1} must be done before P is overwritten or O rescaled
       if (j > 0) ok = ok && mbar_wait_spin(o_done, (j - 1) & 1, abort_flag, p.err, kErrTimeoutEpilogue);
       if (warp == 2 && lane == 0) VAGUS_TRF(j, 8);
-      if (resc && j > 0) {
+      // the tensor-memory loads and stores are the whole warp's: rows that keep their reference scale by 1
+      if (j > 0 && __any_sync(0xffffffffu, resc)) {
         tc_fence_after();
 #pragma unroll
         for (int c = 0; c < D / 64; ++c) {
