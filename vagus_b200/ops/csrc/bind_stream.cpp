@@ -4,6 +4,7 @@
 // tensors' device, on that device's current stream.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <cmath>
@@ -37,6 +38,11 @@ void check(int rc, const char* what) {
 
 bool has(const OptTensor& t) { return t.has_value() && t->defined(); }
 
+// an uninitialised dense tensor, without a trip through the dispatcher (a microsecond a call)
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
+}
+
 int type_of(const Tensor& t, const char* what) {
   const auto s = t.scalar_type();
   TORCH_CHECK_VALUE(s == at::kFloat || s == at::kHalf || s == at::kBFloat16, std::string(what) + ": fp32, fp16 or bf16");
@@ -55,7 +61,7 @@ int index_i64(const Tensor& t, const Tensor& like, const char* what) {
 Tensor unit(const Tensor& t) { return t.stride(-1) == 1 ? t : t.contiguous(); }
 
 // pos: (L,) or (B, L), or none: token l sits at offset + l
-std::vector<Tensor> rotary(Tensor q, OptTensor k, OptTensor pos, int64_t offset, Tensor inv, bool interleaved,
+std::tuple<Tensor, OptTensor> rotary(Tensor q, OptTensor k, OptTensor pos, int64_t offset, Tensor inv, bool interleaved,
                            double scale, double sign) {
   TORCH_CHECK_VALUE(q.is_cuda() && q.dim() == 4, "rotary: q (B, L, H, D)");
   c10::cuda::CUDAGuard guard(q.device());
@@ -64,8 +70,9 @@ std::vector<Tensor> rotary(Tensor q, OptTensor k, OptTensor pos, int64_t offset,
   a.B = q.size(0); a.L = q.size(1); a.H = static_cast<int>(q.size(2)); a.D = static_cast<int>(q.size(3));
   a.q = q.data_ptr();
   a.sq_b = q.stride(0); a.sq_l = q.stride(1); a.sq_h = q.stride(2);
-  std::vector<Tensor> out = {at::empty({a.B, a.L, a.H, a.D}, q.options())};
-  a.yq = out[0].data_ptr();
+  Tensor yq = fresh({a.B, a.L, a.H, a.D}, q.scalar_type(), q);
+  OptTensor yk;
+  a.yq = yq.data_ptr();
   if (has(k)) {
     TORCH_CHECK_VALUE(k->dim() == 4 && k->size(0) == a.B && k->size(1) == a.L && k->size(3) == a.D,
                       "rotary: q (B, L, H, D) and k (B, L, Hk, D)");
@@ -75,8 +82,8 @@ std::vector<Tensor> rotary(Tensor q, OptTensor k, OptTensor pos, int64_t offset,
     a.Hk = static_cast<int>(k->size(2));
     a.k = k->data_ptr();
     a.sk_b = k->stride(0); a.sk_l = k->stride(1); a.sk_h = k->stride(2);
-    out.push_back(at::empty({a.B, a.L, a.Hk, a.D}, q.options()));
-    a.yk = out[1].data_ptr();
+    yk = fresh({a.B, a.L, a.Hk, a.D}, q.scalar_type(), q);
+    a.yk = yk->data_ptr();
   }
   if (has(pos)) {
     a.pos_i64 = index_i64(*pos, q, "rotary: positions");
@@ -99,7 +106,7 @@ std::vector<Tensor> rotary(Tensor q, OptTensor k, OptTensor pos, int64_t offset,
   a.scale = static_cast<float>(scale);
   a.sign = static_cast<float>(sign);
   check(vagus::rotary(a, type_of(q, "rotary"), at::cuda::getCurrentCUDAStream().stream()), "rotary");
-  return out;
+  return {yq, yk};
 }
 
 // ---------------------------------------------------------------- 4-bit KV --
@@ -173,7 +180,7 @@ std::tuple<Tensor, Tensor> kv4_read(Tensor kc, Tensor kp, Tensor vc, Tensor vp, 
   per_row(start, c, a.start, a.start_i64, "int4_read: start");
   TORCH_CHECK_VALUE(count >= 0 && (a.start || (offset >= 0 && offset + count <= c.cap)), "int4_read: tokens [" +
                     str(offset) + ", " + str(offset + count) + ") leave the cache of " + str(c.cap));
-  auto k = at::empty({c.B, c.Hk, count, c.D}, kp.options()), v = at::empty({c.B, c.Hk, count, c.Dv}, kp.options());
+  auto k = fresh({c.B, c.Hk, count, c.D}, at::kBFloat16, kc), v = fresh({c.B, c.Hk, count, c.Dv}, at::kBFloat16, kc);
   a.k_codes = kc.data_ptr(); a.k_params = kp.data_ptr(); a.v_codes = vc.data_ptr(); a.v_params = vp.data_ptr();
   a.k = k.data_ptr(); a.v = v.data_ptr();
   a.offset = offset;
@@ -213,13 +220,28 @@ c10::optional<Tensor> kv4_attn(Tensor q, Tensor kc, Tensor kp, Tensor vc, Tensor
   a.causal = causal ? 1 : 0;
   a.scale_log2 = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(c.D)));
   a.err = vagus_device_error_ptr();
-  auto o = at::empty({c.B, q.size(2), q.size(1), c.Dv}, q.options());
+  auto o = fresh({c.B, q.size(2), q.size(1), c.Dv}, at::kBFloat16, q);
   a.o = o.data_ptr();
   Tensor part;
-  if (o.numel() > 0) {
+  if (vagus::kv4_attn_unpack_first(a)) {
+    auto kv = kv4_read(kc, kp, vc, vp, c10::nullopt, 0, length);
+    const Tensor &k = std::get<0>(kv), &v = std::get<1>(kv);
+    auto lse = fresh({c.B, q.size(1), q.size(2)}, at::kFloat, q);
+    vagus::AttnArgs f;
+    f.q = a.q; f.k = k.data_ptr(); f.v = v.data_ptr(); f.o = a.o; f.lse = lse.data_ptr<float>();
+    f.B = a.B; f.H = a.H; f.Hk = a.Hk; f.Lq = a.Lq; f.Lk = static_cast<int>(length); f.D = a.D; f.Dv = a.Dv;
+    f.sq_b = a.sq_b; f.sq_h = a.sq_h; f.sq_l = a.sq_l;
+    f.sk_b = k.stride(0); f.sk_h = k.stride(1); f.sk_l = k.stride(2);
+    f.sv_b = v.stride(0); f.sv_h = v.stride(1); f.sv_l = v.stride(2);
+    f.so_b = o.stride(0); f.so_h = o.stride(2); f.so_l = o.stride(1);
+    f.causal = a.causal;
+    f.scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(c.D)));
+    f.err = a.err;
+    check(vagus::attn_fwd(f, at::cuda::getCurrentCUDAStream().stream()), "attn_fwd");
+  } else if (o.numel() > 0) {
     check(vagus::kv4_attn_plan(a, a.lengths ? c.cap : length), "kv4_attn");
     if (a.part_rows > 0) {
-      part = at::empty({a.part_rows * (c.Dv + 2)}, q.options().dtype(at::kFloat));
+      part = fresh({a.part_rows * (c.Dv + 2)}, at::kFloat, q);
       a.part_o = part.data_ptr<float>();
       a.part_ml = a.part_o + a.part_rows * c.Dv;
     }
@@ -267,7 +289,7 @@ std::tuple<Tensor, Tensor> verify_draft(Tensor target, OptTensor draft, Tensor t
     lengths = lengths->contiguous();
     a.lengths = lengths->data_ptr();
   }
-  auto out = at::empty({a.B, a.K + 1}, tokens.options()), acc = at::empty({a.B}, tokens.options());
+  auto out = fresh({a.B, a.K + 1}, at::kLong, tokens), acc = fresh({a.B}, at::kLong, tokens);
   a.out = reinterpret_cast<long long*>(out.data_ptr<int64_t>());
   a.accepted = reinterpret_cast<long long*>(acc.data_ptr<int64_t>());
   check(vagus::verify_draft(a, type, at::cuda::getCurrentCUDAStream().stream()),

@@ -243,6 +243,7 @@ struct Kv4AttnArgs {
   int* err;
 };
 int kv4_attn_plan(Kv4AttnArgs& a, long long most_tokens);
+bool kv4_attn_unpack_first(const Kv4AttnArgs& a);           // int4 -> bf16, then attn_fwd
 int kv4_attn(const Kv4AttnArgs& a, cudaStream_t st);
 
 // verify.cu: verification of drafted tokens (see verify.cu).  type: 0 fp32, 1 fp16, 2 bf16.

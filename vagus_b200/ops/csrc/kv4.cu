@@ -41,81 +41,148 @@ __device__ __forceinline__ long long index_at(const void* p, int i64, long long 
   return i64 ? static_cast<const long long*>(p)[i] : static_cast<const int*>(p)[i];
 }
 
+__device__ __forceinline__ uint32_t low2(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x5410); }
+__device__ __forceinline__ uint32_t high2(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
+
 // ---------------------------------------------------------------- append --
 
-// (x - b) / s rounded to the nearest whole number (ties to even).  The product
-// with the reciprocal is within 2^-22 of the quotient's value (at most 143 and a
-// bit), so it rounds alike unless it lies near a half: then, and where the
-// reciprocal is not finite, the quotient is taken.
-__device__ __forceinline__ int code_of(float x, float s, float inv, float b) {
-  const float d = __fsub_rn(x, b), r = d * inv;
-  float k = rintf(r);
-  if (!(fabsf(r - k) < 0.499f)) k = rintf(__fdiv_rn(d, s));
-  const int c = __float2int_rn(fminf(fmaxf(k, 128.f), 143.f)) - 128;
-  return s > 0.f ? c : 0;
+// The codes of 16 channels by their definition: (x - b) / s rounded to the nearest whole
+// number (ties to even), less 128.
+__device__ __noinline__ uint2 codes_by_division(const float* x, float s, float b) {
+  uint32_t w[2] = {0u, 0u};
+#pragma unroll 1
+  for (int j = 15; j >= 0; --j) {
+    const float k = rintf(__fdiv_rn(__fsub_rn(x[j], b), s));
+    const uint32_t c = s > 0.f ? static_cast<uint32_t>(__float2int_rn(fminf(fmaxf(k, 128.f), 143.f)) - 128) : 0u;
+    w[j / 8] = w[j / 8] * 16u + c;
+  }
+  return make_uint2(w[0], w[1]);
 }
 
-// 8 channels a thread, 4 threads a group of 32; rows (b, l, h) in the order the
-// projections leave them, so the reads are contiguous.
-template <typename T, bool VEC>
+// The same in full-rate operations, nine a channel.  q0 = d r with the correctly rounded
+// reciprocal r of s, corrected once by its exact remainder, is the correctly rounded d / s
+// (Markstein); outside the range of s where neither over- nor underflows, by division.
+// (Checking d r for being near to a half and dividing only then took a branch in two warps
+// out of three, since a bf16 x lies exactly half way in one case of 500: 254 us against
+// 115 for 4 x 8191 tokens of 16 heads.)  Adding and subtracting 1.5 * 2^23 rounds to a whole
+// number, ties to even; four codes are gathered as one float, whose low 16 bits they are
+// once 2^23 is added.
+__device__ __forceinline__ uint2 codes_of(const float (&x)[16], float s, float b) {
+  constexpr float kRound = 12582912.f, kGather = 8388608.f - 128.f * 4369.f;      // 4369 = 1 + 16 + 256 + 4096
+  if (!(s > 1e-30f && s < 1e36f)) {
+    float y[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) y[j] = x[j];
+    return codes_by_division(y, s, b);
+  }
+  const float r = __frcp_rn(s);
+  uint32_t four[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 3; j >= 0; --j) {
+      const float d = __fsub_rn(x[4 * q + j], b), q0 = __fmul_rn(d, r), t = fmaf(fmaf(-q0, s, d), r, q0);
+      const float c = (fminf(fmaxf(t, 128.f), 143.f) + kRound) - kRound;
+      sum = j == 3 ? c : fmaf(sum, 16.f, c);
+    }
+    four[q] = __float_as_uint(sum + kGather);
+  }
+  return make_uint2(low2(four[0], four[1]), low2(four[2], four[3]));
+}
+
+// x / 15 correctly rounded: the product with 1 / 15, corrected once by its exact remainder
+// (by division outside the range where that holds).
+__device__ __forceinline__ float fifteenth(float x) {
+  if (!(x > 1e-30f && x < 1e37f)) return __fdiv_rn(x, 15.f);
+  constexpr float c = 1.f / 15.f;
+  const float q = x * c;
+  return fmaf(fmaf(-15.f, q, x), c, q);
+}
+
+// 16 channels a thread, 2 threads a group of 32, ROWS rows a thread.  Rows go in the order
+// (token, head) in which the projections leave them, so the reads are contiguous.  Bound by
+// the arithmetic of the codes: 3.4 TB/s for 4 x 8191 tokens of 16 heads of 128 (104 us; its
+// reads and writes alone would take 54), with every issue slot in three used.
+template <typename T, bool VEC, int ROWS>
 __global__ void __launch_bounds__(256) kv4_append_k(const Kv4AppendArgs a) {
-  const int which = blockIdx.y;                       // 0: keys, 1: values
-  const int D = which ? a.Dv : a.D, per = D / 8;
-  const T* x = static_cast<const T*>(which ? a.v : a.k);
-  const long long sb = which ? a.sv_b : a.sk_b, sh = which ? a.sv_h : a.sk_h, sl = which ? a.sv_l : a.sk_l;
-  const long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
-  const long long row = i / per, total = a.B * a.L * a.Hk;
-  const bool live = row < total;                      // whole groups of 4 threads are live or not
-  const int c0 = static_cast<int>(i - row * per) * 8;
-  const long long bl = row / a.Hk, b = bl / a.L;
-  const long long l = bl - b * a.L, h = row - bl * a.Hk;
-  float v[8];
+  const int which = blockIdx.z;                       // 0: keys, 1: values
+  const int D = which ? a.Dv : a.D, per = D / 16, rows = 256 / per;
+  const int ty = threadIdx.x / per, part = threadIdx.x - ty * per;
+  const long long b = blockIdx.y;
+  const T* x = static_cast<const T*>(which ? a.v : a.k) + b * (which ? a.sv_b : a.sk_b) + 16 * part;
+  const long long sh = which ? a.sv_h : a.sk_h, sl = which ? a.sv_l : a.sk_l;
+  const unsigned total = static_cast<unsigned>(a.L) * a.Hk, Hk = a.Hk, r0 = blockIdx.x * (rows * ROWS) + ty;
+  const long long start = a.start ? index_at(a.start, a.start_i64, b) : a.offset;
+  const bool idle = ty >= rows;                       // threads past the last whole row of threads
+
+  // token and head of each row, by one division
+  unsigned ls[ROWS], hs[ROWS];
+  const unsigned dl = rows / Hk, dh = rows - dl * Hk;
+  ls[0] = r0 / Hk;
+  hs[0] = r0 - ls[0] * Hk;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = 0.f;
-  if (live) {
-    const T* p = x + b * sb + h * sh + l * sl + c0;
-    if (VEC) {
-      constexpr int N = 16 / sizeof(T);
-#pragma unroll
-      for (int j = 0; j < 8; j += N) {
-        const uint4 u = *reinterpret_cast<const uint4*>(p + j);
-        const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-        for (int k = 0; k < N; ++k) v[j + k] = to_f(e[k]);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = to_f(p[j]);
+  for (int i = 1; i < ROWS; ++i) {
+    ls[i] = ls[i - 1] + dl;
+    hs[i] = hs[i - 1] + dh;
+    if (hs[i] >= Hk) {
+      hs[i] -= Hk;
+      ++ls[i];
     }
   }
-  float lo = v[0], hi = v[0];
+  constexpr int N = 16 / sizeof(T);                   // elements a 16-byte load
+  uint4 raw[VEC ? ROWS : 1][16 / N];
+  if (VEC) {
 #pragma unroll
-  for (int j = 1; j < 8; ++j) { lo = min_nan(lo, v[j]); hi = max_nan(hi, v[j]); }
+    for (int i = 0; i < ROWS; ++i) {
+      if (!idle && r0 + i * rows < total) {
 #pragma unroll
-  for (int o = 1; o < 4; o <<= 1) {
-    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        for (int j = 0; j < 16 / N; ++j) raw[i][j] = *reinterpret_cast<const uint4*>(x + hs[i] * sh + ls[i] * sl + j * N);
+      }
+    }
   }
-  if (!live) return;
-  const long long t = l + (a.start ? index_at(a.start, a.start_i64, b) : a.offset);
-  if (t < 0 || t >= a.cap) {                          // a start given on the device that leaves the cache
-    record_error(a.err, kErrBadArgument);
-    return;
-  }
-  const __nv_bfloat16 s16 = __float2bfloat16_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.f));
-  const float s = __bfloat162float(s16);
-  const __nv_bfloat16 b16 = __float2bfloat16_rn(__fsub_rn(lo, __fmul_rn(128.f, s)));
-  const float off = __bfloat162float(b16), inv = __frcp_rn(s);
-  uint32_t w = 0;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) w |= static_cast<uint32_t>(code_of(v[j], s, inv, off)) << (4 * j);
-  const long long out = (b * a.Hk + h) * a.cap + t;
-  uint32_t* codes = reinterpret_cast<uint32_t*>(which ? a.v_codes : a.k_codes);
-  codes[out * per + c0 / 8] = w;
-  if ((c0 & (kGroup - 1)) == 0) {
-    const __nv_bfloat162 pr = __halves2bfloat162(s16, b16);
-    uint32_t* params = reinterpret_cast<uint32_t*>(which ? a.v_params : a.k_params);
-    params[out * (D / kGroup) + c0 / kGroup] = *reinterpret_cast<const uint32_t*>(&pr);
+  for (int i = 0; i < ROWS; ++i) {
+    const unsigned l = ls[i], h = hs[i];
+    const bool live = !idle && r0 + i * rows < total;         // pairs of threads are live or not together
+    float v[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = 0.f;
+    if (live) {
+      if (VEC) {
+#pragma unroll
+        for (int j = 0; j < 16 / N; ++j) {
+          const T* e = reinterpret_cast<const T*>(&raw[i][j]);
+#pragma unroll
+          for (int k = 0; k < N; ++k) v[j * N + k] = to_f(e[k]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = to_f(x[h * sh + l * sl + j]);
+      }
+    }
+    float lo = v[0], hi = v[0];
+#pragma unroll
+    for (int j = 1; j < 16; ++j) { lo = min_nan(lo, v[j]); hi = max_nan(hi, v[j]); }
+    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, 1));
+    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, 1));
+    if (!live) continue;
+    const long long t = start + l;
+    if (t < 0 || t >= a.cap) {                        // a start given on the device that leaves the cache
+      record_error(a.err, kErrBadArgument);
+      continue;
+    }
+    const __nv_bfloat16 s16 = __float2bfloat16_rn(fifteenth(__fsub_rn(hi, lo)));
+    const float s = __bfloat162float(s16);
+    const __nv_bfloat16 b16 = __float2bfloat16_rn(__fsub_rn(lo, __fmul_rn(128.f, s)));
+    const uint2 w = codes_of(v, s, __bfloat162float(b16));
+    const long long out = (b * a.Hk + h) * a.cap + t;
+    reinterpret_cast<uint2*>(which ? a.v_codes : a.k_codes)[out * per + part] = w;
+    if ((part & 1) == 0) {
+      const __nv_bfloat162 pr = __halves2bfloat162(s16, b16);
+      reinterpret_cast<uint32_t*>(which ? a.v_params : a.k_params)[out * (D / kGroup) + part / 2] =
+          *reinterpret_cast<const uint32_t*>(&pr);
+    }
   }
 }
 
@@ -135,34 +202,66 @@ __device__ __forceinline__ uint32_t pair_of(uint32_t w, uint32_t ss, uint32_t bb
   asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;" : "=r"(x) : "r"(w >> (4 * I)), "r"(magic));   // (w & mask) | magic
   return fma_bf16x2(x, ss, bb);
 }
-__device__ __forceinline__ uint32_t low2(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x5410); }
-__device__ __forceinline__ uint32_t high2(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
+__device__ __forceinline__ uint4 unpack(uint32_t w, uint32_t p, uint32_t magic) {
+  const uint32_t ss = low2(p, p), bb = high2(p, p);
+  const uint32_t p0 = pair_of<0>(w, ss, bb, magic), p1 = pair_of<1>(w, ss, bb, magic), p2 = pair_of<2>(w, ss, bb, magic),
+                 p3 = pair_of<3>(w, ss, bb, magic);
+  return make_uint4(low2(p0, p1), low2(p2, p3), high2(p0, p1), high2(p2, p3));
+}
 
-// 8 channels a thread: 4 bytes of codes in, 16 bytes of values out
-__global__ void __launch_bounds__(256) kv4_read_k(const Kv4ReadArgs a) {
-  const int which = blockIdx.y;
-  const int D = which ? a.Dv : a.D, per = D / 8;
-  const uint32_t* codes = reinterpret_cast<const uint32_t*>(which ? a.v_codes : a.k_codes);
-  const uint32_t* params = reinterpret_cast<const uint32_t*>(which ? a.v_params : a.k_params);
-  uint4* out = reinterpret_cast<uint4*>(which ? a.v : a.k);
-  const long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
-  const long long row = i / per;
-  if (row >= a.B * a.Hk * a.L) return;
-  const int cw = static_cast<int>(i - row * per);
-  const long long bh = row / a.L, l = row - bh * a.L, b = bh / a.Hk;
-  const long long t = l + (a.start ? index_at(a.start, a.start_i64, b) : a.offset);
+// A head's tokens lie one after the other in the codes, the parameters and the result, so
+// word i of its codes goes with parameter i / 4 and becomes 16-byte vector i of the result.
+// 8 words a thread, loaded at once; bound by its reads and writes.
+constexpr int kReadWords = 8;
+__global__ void __launch_bounds__(256) kv4_read_k(const Kv4ReadArgs a, unsigned blocks_k) {
+  // the first blocks take the keys, the others the values
+  const int which = blockIdx.x >= blocks_k;
+  const unsigned block = which ? blockIdx.x - blocks_k : blockIdx.x;
+  const int D = which ? a.Dv : a.D;
+  const long long words = a.L * (D / 8);
+  const unsigned per_head = static_cast<unsigned>((words + 256 * kReadWords - 1) / (256 * kReadWords));
+  const unsigned bh = block / per_head;
+  const long long i0 = static_cast<long long>(block - bh * per_head) * (256 * kReadWords) + threadIdx.x;
+  const long long start = a.start ? index_at(a.start, a.start_i64, bh / a.Hk) : a.offset;
+  const long long at = static_cast<long long>(bh) * a.cap + start;
+  const uint32_t* codes = reinterpret_cast<const uint32_t*>(which ? a.v_codes : a.k_codes) + at * (D / 8);
+  const uint32_t* params = reinterpret_cast<const uint32_t*>(which ? a.v_params : a.k_params) + at * (D / kGroup);
+  uint4* out = reinterpret_cast<uint4*>(which ? a.v : a.k) + bh * words;
+  // a start given on the device may leave the cache: tokens outside read as zeros
+  long long lo = 0, hi = words;
+  if (start < 0 || start + a.L > a.cap) {
+    if (threadIdx.x == 0) record_error(a.err, kErrBadArgument);
+    lo = start < 0 ? -start * (D / 8) : 0;
+    hi = (a.cap - start) * (D / 8);
+  }
+  uint32_t w[kReadWords], p[kReadWords];
+#pragma unroll
+  for (int j = 0; j < kReadWords; ++j) {
+    const long long i = i0 + 256 * j;
+    w[j] = p[j] = 0u;
+    if (i < words && i >= lo && i < hi) { w[j] = codes[i]; p[j] = params[i / 4]; }
+  }
+#pragma unroll
+  for (int j = 0; j < kReadWords; ++j)
+    if (i0 + 256 * j < words) out[i0 + 256 * j] = unpack(w[j], p[j], a.magic);
+}
+
+// Few tokens: a word a thread, over the heads of all sequences.
+__global__ void __launch_bounds__(256) kv4_read_few_k(const Kv4ReadArgs a) {
+  const int which = blockIdx.y, D = which ? a.Dv : a.D;
+  const unsigned words = static_cast<unsigned>(a.L) * (D / 8), i = blockIdx.x * 256 + threadIdx.x, bh = i / words;
+  if (bh >= a.B * a.Hk) return;
+  const unsigned iw = i - bh * words, l = iw / (D / 8);
+  const long long t = l + (a.start ? index_at(a.start, a.start_i64, bh / a.Hk) : a.offset);
+  uint4 x = make_uint4(0, 0, 0, 0);
   if (t < 0 || t >= a.cap) {
     record_error(a.err, kErrBadArgument);
-    out[i] = make_uint4(0, 0, 0, 0);
-    return;
+  } else {
+    const long long at = (bh * a.cap + t) * (D / 8) + (iw - l * (D / 8));
+    x = unpack(reinterpret_cast<const uint32_t*>(which ? a.v_codes : a.k_codes)[at],
+               reinterpret_cast<const uint32_t*>(which ? a.v_params : a.k_params)[at / 4], a.magic);
   }
-  const long long at = bh * a.cap + t;
-  const uint32_t w = codes[at * per + cw], p = params[at * (D / kGroup) + cw / 4];
-  const uint32_t ss = low2(p, p), bb = high2(p, p);
-  const uint32_t un = a.magic;
-  const uint32_t p0 = pair_of<0>(w, ss, bb, un), p1 = pair_of<1>(w, ss, bb, un), p2 = pair_of<2>(w, ss, bb, un),
-                 p3 = pair_of<3>(w, ss, bb, un);
-  out[i] = make_uint4(low2(p0, p1), low2(p2, p3), high2(p0, p1), high2(p2, p3));
+  reinterpret_cast<uint4*>(which ? a.v : a.k)[i] = x;
 }
 
 // ------------------------------------------------------------- attention --
@@ -782,18 +881,24 @@ int attn_launch(const Kv4AttnArgs& a, cudaStream_t st) {
 }  // namespace
 
 int kv4_append(const Kv4AppendArgs& a, int type, cudaStream_t st) {
-  if (a.D % kGroup || a.Dv % kGroup || a.D < kGroup || a.Dv < kGroup) return 1;
+  if (a.D % kGroup || a.Dv % kGroup || a.D < kGroup || a.Dv < kGroup || a.D > 4096 || a.Dv > 4096) return 1;
   if (a.B * a.L * a.Hk == 0) return 0;
-  const long long most = a.B * a.L * a.Hk * ((a.D > a.Dv ? a.D : a.Dv) / 8), blocks = (most + 255) / 256;
-  if (blocks > 0x7fffffffLL) return 2;
-  const dim3 grid(static_cast<unsigned>(blocks), 2);
+  const int widest = a.D > a.Dv ? a.D : a.Dv, rows = 256 / (widest / 16);     // rows a block takes at once
+  if (a.L * a.Hk > 0x7fffffffLL - 4096 || a.B > 65535) return 2;
+  // four rows a thread, whose loads overlap, once that still makes several blocks an SM; one row below (300 tokens
+  // of 16 heads of 64: 2.6 us against 4.1)
+  const int each = a.B * ((a.L * a.Hk + 4 * rows - 1) / (4 * rows)) >= 148 * 4 ? 4 : 1;
+  const dim3 grid(static_cast<unsigned>((a.L * a.Hk + each * rows - 1) / (each * rows)), static_cast<unsigned>(a.B), 2);
   const int es = type == 0 ? 4 : 2;
   auto al = [es](const void* p, long long x, long long y, long long z) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && x * es % 16 == 0 && y * es % 16 == 0 && z * es % 16 == 0;
   };
   const bool vec = al(a.k, a.sk_b, a.sk_h, a.sk_l) && al(a.v, a.sv_b, a.sv_h, a.sv_l);
-#define VAGUS_KV4_APPEND(T) \
-  if (vec) kv4_append_k<T, true><<<grid, 256, 0, st>>>(a); else kv4_append_k<T, false><<<grid, 256, 0, st>>>(a)
+#define VAGUS_KV4_APPEND(T)                                              \
+  if (vec && each == 4) kv4_append_k<T, true, 4><<<grid, 256, 0, st>>>(a); \
+  else if (vec) kv4_append_k<T, true, 1><<<grid, 256, 0, st>>>(a);        \
+  else if (each == 4) kv4_append_k<T, false, 4><<<grid, 256, 0, st>>>(a); \
+  else kv4_append_k<T, false, 1><<<grid, 256, 0, st>>>(a)
   if (type == 0) { VAGUS_KV4_APPEND(float); }
   else if (type == 1) { VAGUS_KV4_APPEND(__half); }
   else { VAGUS_KV4_APPEND(__nv_bfloat16); }
@@ -804,10 +909,18 @@ int kv4_append(const Kv4AppendArgs& a, int type, cudaStream_t st) {
 int kv4_read(Kv4ReadArgs a, cudaStream_t st) {
   if (a.D % kGroup || a.Dv % kGroup || a.D < kGroup || a.Dv < kGroup) return 1;
   if (a.B * a.L * a.Hk == 0) return 0;
-  const long long most = a.B * a.L * a.Hk * ((a.D > a.Dv ? a.D : a.Dv) / 8), blocks = (most + 255) / 256;
-  if (blocks > 0x7fffffffLL) return 2;
   a.magic = 0x43004300u;
-  kv4_read_k<<<dim3(static_cast<unsigned>(blocks), 2), 256, 0, st>>>(a);
+  // fewer words a head than a block of the first kernel takes (one token of 64 sequences of 8 heads: 1.9 us
+  // against 4.6 with a block a head)
+  const long long widest = a.L * ((a.D > a.Dv ? a.D : a.Dv) / 8), flat = a.B * a.Hk * widest;
+  if (widest < 256 * kReadWords && flat < 0x7fffff00LL) {
+    kv4_read_few_k<<<dim3(static_cast<unsigned>((flat + 255) / 256), 2), 256, 0, st>>>(a);
+    return cudaGetLastError() == cudaSuccess ? 0 : 3;
+  }
+  auto blocks = [&](int D) { return a.B * a.Hk * ((a.L * (D / 8) + 256 * kReadWords - 1) / (256 * kReadWords)); };
+  const long long k = blocks(a.D), v = blocks(a.Dv);
+  if (k + v > 0x7fffffffLL) return 2;
+  kv4_read_k<<<static_cast<unsigned>(k + v), 256, 0, st>>>(a, static_cast<unsigned>(k));
   return cudaGetLastError() == cudaSuccess ? 0 : 3;
 }
 
@@ -834,6 +947,20 @@ int kv4_attn_plan(Kv4AttnArgs& a, long long most_tokens) {
     }
   }
   return 0;
+}
+
+// Whether many query rows over equal lengths are better served by unpacking the values once and running the
+// tcgen05 attention on them.  The kernels above take 5.2 ns a unit and tile of 16 rows, on the whole GPU; the
+// other way takes the read, some 12 us of launches and, a wave of 128-row CTAs, 1.5 us per 128 tokens.  Measured, 16
+// heads of 128 over 8192 tokens: 55 / 177 / 341 us against 109 / 109 / 111 at 128 / 512 / 1024 rows; over 32768
+// tokens of 16 heads of 64: 103 / 377 / 741 against 381 / 383 / 385.
+bool kv4_attn_unpack_first(const Kv4AttnArgs& a) {
+  if (a.lengths || a.Lq < 128 || a.length < 128 || a.Lq > a.length || a.D != a.Dv) return false;
+  const double tiles = (static_cast<double>(a.H / a.Hk) * a.Lq + 15) / 16, units = (a.length + kUnit - 1) / kUnit;
+  const double here = 0.0052 * a.B * a.Hk * tiles * units;
+  const long long ctas = a.B * a.H * ((a.Lq + 127) / 128), wave = a.D == 64 ? 296 : 148;
+  const double there = 12 + 5e-7 * a.B * a.Hk * a.length * (a.D + a.Dv) + 1.5 * ((ctas + wave - 1) / wave) * units;
+  return there < here;
 }
 
 int kv4_attn(const Kv4AttnArgs& a, cudaStream_t st) {

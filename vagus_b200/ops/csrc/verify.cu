@@ -14,15 +14,15 @@
 // requests: two dependent reads (the drafted tokens, their probabilities) before
 // the row is known.  A cluster of CTAs takes a row, each warp one contiguous
 // piece of it: one pass for the pieces' sums, which meet through distributed
-// shared memory, then the warp whose piece holds the border goes over that piece
-// again (it is in L2) to find the token.
+// shared memory, then the CTA whose piece holds the border goes over that piece again
+// (it is in L2), a part a warp, and the warp whose part holds it finds the token.
 #include "common.cuh"
 #include "kernels.h"
 
 namespace vagus {
 namespace {
 
-constexpr int kWarps = 16, kThreads = 32 * kWarps, kMaxCluster = 8;
+constexpr int kWarps = 8, kThreads = 32 * kWarps, kMaxCluster = 8;
 
 template <typename T> __device__ __forceinline__ float to_f(T v);
 template <> __device__ __forceinline__ float to_f(float v) { return v; }
@@ -77,9 +77,25 @@ __device__ __forceinline__ void four(const Row<T>& r, long long v, long long hi,
   }
 }
 
+// sum of the weights lo .. hi - 1 over a warp; kAhead vectors of each row under way
+constexpr int kAhead = 4;
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kThreads) verify_k(const VerifyArgs a) {
-  __shared__ double warp_total[kWarps];
+__device__ __forceinline__ double sum_of(const Row<T>& r, long long lo, long long hi, int lane) {
+  double s = 0;
+  for (long long v = lo + 4 * lane; v < hi; v += 128 * kAhead) {
+    float w[kAhead][4];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) four<T, VEC>(r, v + 128 * j, hi, w[j]);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      s += (static_cast<double>(w[j][0]) + w[j][1]) + (static_cast<double>(w[j][2]) + w[j][3]);
+  }
+  return warp_sum_f64(s);
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kThreads, 4) verify_k(const VerifyArgs a) {
+  __shared__ double warp_total[kWarps], part_total[kWarps];
   __shared__ double cta_total;
   __shared__ int s_acc;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -125,13 +141,7 @@ __global__ void __launch_bounds__(kThreads) verify_k(const VerifyArgs a) {
 
   double before = 0, total = 0, totals[kMaxCluster];
   for (int pass = 0; pass < 2; ++pass) {
-    double s = 0;
-    for (long long v = lo + 4 * lane; v < hi; v += 128) {
-      float w[4];
-      four<T, VEC>(row, v, hi, w);
-      s += (static_cast<double>(w[0]) + w[1]) + (static_cast<double>(w[2]) + w[3]);
-    }
-    s = warp_sum_f64(s);
+    const double s = sum_of<T, VEC>(row, lo, hi, lane);
     if (lane == 0) warp_total[warp] = s;
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -168,23 +178,35 @@ __global__ void __launch_bounds__(kThreads) verify_k(const VerifyArgs a) {
     at += mine;
   }
   if (rank != (owner < 0 ? 0 : owner)) return;
-  int owner_warp = -1;
-  double base = 0;
-  at = before;
-  for (int w = 0; w < kWarps; ++w) {
-    const double mine = warp_total[w];
-    if (mine > 0 && !(at > t)) { owner_warp = w; base = at; }
-    at += mine;
-  }
-  if (warp != (owner_warp < 0 ? 0 : owner_warp)) return;
-
+  // The same again for the pieces of this CTA's warps, then for the parts of that piece, one a warp.
+  auto last_below = [&](const double* sums, double& base) {
+    int found = -1;
+    double run = base;
+    for (int w = 0; w < kWarps; ++w) {
+      const double mine = sums[w];
+      if (mine > 0 && !(run > t)) { found = w; base = run; }
+      run += mine;
+    }
+    return found;
+  };
+  double base = before;
+  const int piece_at = last_below(warp_total, base);
   long long token = 0;                 // a row without any weight gives token 0
-  if (owner_warp >= 0) {
+  if (piece_at >= 0) {
+    const long long plo = min(a.V, (static_cast<long long>(rank) * kWarps + piece_at) * piece), phi = min(a.V, plo + piece);
+    const long long part = (piece / 128 + kWarps - 1) / kWarps * 128;
+    const long long qlo = min(phi, plo + warp * part), qhi = min(phi, qlo + part);
+    const double s = sum_of<T, VEC>(row, qlo, qhi, lane);
+    if (lane == 0) part_total[warp] = s;
+    __syncthreads();
+    int mine = last_below(part_total, base);
+    if (mine < 0) mine = 0;            // rounding left the piece nothing below: its first part
+    if (warp != mine) return;
     long long found = -1, last = -1;
-    for (long long v0 = lo; v0 < hi && found < 0; v0 += 128) {
+    for (long long v0 = qlo; v0 < qhi && found < 0; v0 += 128) {
       const long long v = v0 + 4 * lane;
       float w[4];
-      four<T, VEC>(row, v, hi, w);
+      four<T, VEC>(row, v, qhi, w);
       double in[4];                    // running sums of this lane's four, the lane's first included
       in[0] = w[0];
 #pragma unroll
@@ -213,6 +235,8 @@ __global__ void __launch_bounds__(kThreads) verify_k(const VerifyArgs a) {
       base += __shfl_sync(0xffffffffu, scan, 31);
     }
     token = found >= 0 ? found : last;
+  } else if (warp != 0) {
+    return;
   }
   for (int i = lane; i <= a.K; i += 32)
     a.out[b * (a.K + 1) + i] = i < acc ? tok[i] : i == acc ? token : -1;

@@ -52,8 +52,7 @@ class _Rotary(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(pos, inv)
         ctx.meta = (offset, interleaved, scale, sign)
-        out = native().rotary(q, k, pos, offset, inv, interleaved, scale, sign)
-        return out[0], (out[1] if k is not None else None)
+        return native().rotary(q, k, pos, offset, inv, interleaved, scale, sign)
 
     @staticmethod
     def backward(ctx, dq, dk):
@@ -61,17 +60,12 @@ class _Rotary(torch.autograd.Function):
         offset, interleaved, scale, sign = ctx.meta
         if dq is None and dk is None:
             return (None,) * 8
-        run = _Rotary.apply if torch.is_grad_enabled() else _run
+        run = _Rotary.apply if torch.is_grad_enabled() else native().rotary
         if dq is None:
             gk, gq = run(dk, None, pos, offset, inv, interleaved, scale, -sign)
         else:
             gq, gk = run(dq, dk, pos, offset, inv, interleaved, scale, -sign)
         return gq, gk, None, None, None, None, None, None
-
-
-def _run(q, k, *rest):
-    out = native().rotary(q, k, *rest)
-    return out if k is not None else (out[0], None)
 
 
 def _check(q, k, positions, inv_freq):
@@ -110,7 +104,8 @@ def rotary(q, k, positions, inv_freq, layout: str = "interleaved", scale: float 
         y = rotary_ref(q, positions, inv_freq, layout, scale)
         return y if k is None else (y, rotary_ref(k, positions, inv_freq, layout, scale))
     # on the GPU the binding checks the arguments (the same conditions)
-    graph = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
-    run = _Rotary.apply if graph else _run
-    yq, yk = run(q, k, pos, offset, inv_freq.detach(), layout == "interleaved", scale, 1.0)
-    return yq if k is None else (yq, yk)
+    run = native().rotary
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        run = _Rotary.apply
+    out = run(q, k, pos, offset, inv_freq, layout == "interleaved", scale, 1.0)
+    return out[0] if k is None else out
