@@ -66,15 +66,16 @@ __device__ __forceinline__ void row_of(const RotaryArgs& a, long long b, long lo
   }
 }
 
-// blockDim = (items of a head, heads); an item is one 16-byte vector, or for the half
+// blockDim = (items of a head, rows); the rows are `across` heads of one token or, where the
+// heads are few, of several; an item is one 16-byte vector, or for the half
 // layout's rotated channels the two vectors that pair up.  The angles of an item's P pairs
 // are read as float4s of two; those lie [which of the P / 2][item], so that neighbouring
-// threads read neighbouring 16 bytes (item-major, 8 threads met in 2 of 8 bank groups: 116
-// us against 113 for both directions of 4 x 4096 tokens of 32 heads of 128).  Full
-// occupancy matters more than loads held ahead in registers: 99 us at 32 registers, 113 at
-// 40, 120 to 187 with two to four rows' loads first.  5.4 TB/s.
+// threads read neighbouring 16 bytes (item-major, 8 threads met in 2 of 8 bank groups).
+// Many resident threads matter more than loads held ahead in registers: two to four rows'
+// loads first took 146 to 187 us instead of 99 for both directions of 4 x 4096 tokens of 32
+// heads of 128 in bf16 (5.3 TB/s; fp32 6.2 TB/s).
 template <typename T, bool INTER>
-__global__ void __launch_bounds__(kThreads, 8) rotary_vec_k(const RotaryArgs a, int tokens) {
+__global__ void __launch_bounds__(kThreads, INTER ? 8 : 6) rotary_vec_k(const RotaryArgs a, int tokens, int across) {
   constexpr int N = Vec<T>::N, P = INTER ? N / 2 : N;
   extern __shared__ __align__(16) float2 cs[];                    // [tokens][R / 2]
   __shared__ long long q_at[kThreads], k_at[kThreads];            // where a token's heads begin
@@ -97,17 +98,18 @@ __global__ void __launch_bounds__(kThreads, 8) rotary_vec_k(const RotaryArgs a, 
   const int rot = INTER ? a.R / N : half / N;                     // items that rotate
   const bool pair = !INTER && item < rot;
   const int c0 = INTER || pair ? item * N : a.R + (item - rot) * N;
-  for (int tk = 0; tk < nt; ++tk) {
-    const long long t = t0 + tk;
-    const float4* c = reinterpret_cast<const float4*>(cs + tk * half) + item;
-    const T* q = static_cast<const T*>(a.q) + q_at[tk] + c0;
-    const T* k = static_cast<const T*>(a.k) + k_at[tk] + c0;
-    T* yq = static_cast<T*>(a.yq) + t * a.H * a.D + c0;
-    T* yk = static_cast<T*>(a.yk) + t * a.Hk * a.D + c0;
+  const int ty = threadIdx.y / across, tstep = blockDim.y / across;
+  for (int h = threadIdx.y - ty * across; h < heads; h += across) {
+    const bool is_q = h < a.H;
+    const T* in = is_q ? static_cast<const T*>(a.q) + h * a.sq_h : static_cast<const T*>(a.k) + (h - a.H) * a.sk_h;
+    const long long* at = is_q ? q_at : k_at;
+    const long long pitch = static_cast<long long>(is_q ? a.H : a.Hk) * a.D;
+    T* out = (is_q ? static_cast<T*>(a.yq) + h * a.D : static_cast<T*>(a.yk) + (h - a.H) * a.D) + t0 * pitch;
 #pragma unroll 2
-    for (int h = threadIdx.y; h < heads; h += blockDim.y) {
-      const T* src = h < a.H ? q + h * a.sq_h : k + (h - a.H) * a.sk_h;
-      T* dst = h < a.H ? yq + h * a.D : yk + (h - a.H) * a.D;
+    for (int tk = ty; tk < nt; tk += tstep) {
+      const float4* c = reinterpret_cast<const float4*>(cs + tk * half) + item;
+      const T* src = in + at[tk] + c0;
+      T* dst = out + tk * pitch + c0;
       Vec<T> x = *reinterpret_cast<const Vec<T>*>(src);
       if (INTER) {
         if (item < rot) {
@@ -192,9 +194,12 @@ int launch(const RotaryArgs& a, cudaStream_t st) {
                    a.D % N == 0 && (a.interleaved ? a.R % N == 0 : half % N == 0);
   const int items = vec ? (a.interleaved ? a.D / N : half / N + (a.D - a.R) / N) : 0;
   if (vec && items <= kThreads) {
-    const dim3 block(items, kThreads / items);
-    if (a.interleaved) rotary_vec_k<T, true><<<static_cast<unsigned>(grid), block, smem, st>>>(a, tokens);
-    else rotary_vec_k<T, false><<<static_cast<unsigned>(grid), block, smem, st>>>(a, tokens);
+    // rows: all heads of as many tokens as fit, or an even share of the heads of one
+    const int room = kThreads / items, heads = a.H + a.Hk, turns = (heads + room - 1) / room;
+    const int across = (heads + turns - 1) / turns, each = turns > 1 ? 1 : room / heads;
+    const dim3 block(items, across * (each < tokens ? each : tokens));
+    if (a.interleaved) rotary_vec_k<T, true><<<static_cast<unsigned>(grid), block, smem, st>>>(a, tokens, across);
+    else rotary_vec_k<T, false><<<static_cast<unsigned>(grid), block, smem, st>>>(a, tokens, across);
   } else {
     rotary_any_k<T><<<static_cast<unsigned>(grid), kThreads, smem, st>>>(a, tokens);
   }
