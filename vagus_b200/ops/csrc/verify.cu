@@ -77,18 +77,39 @@ __device__ __forceinline__ void four(const Row<T>& r, long long v, long long hi,
   }
 }
 
-// sum of the weights lo .. hi - 1 over a warp; kAhead vectors of each row under way
+// Sum of the weights lo .. hi - 1 over a warp: whole stretches with kAhead vectors of each
+// row under way (their loads in front of everything that branches), then the rest.
 constexpr int kAhead = 4;
+template <typename T, bool HAS_Q>
+__device__ __forceinline__ double sum_whole(const Row<T>& r, long long& v, long long hi) {
+  double s = 0;
+  for (; v - 4 * (threadIdx.x % 32) + 128 * kAhead <= hi; v += 128 * kAhead) {
+    Quad<T> p[kAhead], q[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      p[j] = *reinterpret_cast<const Quad<T>*>(r.p + v + 128 * j);
+      if (HAS_Q) q[j] = *reinterpret_cast<const Quad<T>*>(r.q + v + 128 * j);
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      float w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = r.weight(v + 128 * j + e, to_f(p[j].v[e]), HAS_Q ? to_f(q[j].v[e]) : 0.f);
+      s += (static_cast<double>(w[0]) + w[1]) + (static_cast<double>(w[2]) + w[3]);
+    }
+  }
+  return s;
+}
+
 template <typename T, bool VEC>
 __device__ __forceinline__ double sum_of(const Row<T>& r, long long lo, long long hi, int lane) {
   double s = 0;
-  for (long long v = lo + 4 * lane; v < hi; v += 128 * kAhead) {
-    float w[kAhead][4];
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) four<T, VEC>(r, v + 128 * j, hi, w[j]);
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j)
-      s += (static_cast<double>(w[j][0]) + w[j][1]) + (static_cast<double>(w[j][2]) + w[j][3]);
+  long long v = lo + 4 * lane;
+  if (VEC) s = r.q ? sum_whole<T, true>(r, v, hi) : sum_whole<T, false>(r, v, hi);
+  for (; v < hi; v += 128) {
+    float w[4];
+    four<T, VEC>(r, v, hi, w);
+    s += (static_cast<double>(w[0]) + w[1]) + (static_cast<double>(w[2]) + w[3]);
   }
   return warp_sum_f64(s);
 }
