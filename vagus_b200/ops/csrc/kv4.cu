@@ -727,12 +727,12 @@ __global__ void __launch_bounds__(32 * kAttnWarps, ctas_per_sm(NT)) kv4_attn_k(c
   }
 }
 
-// One CTA a row of an item whose units several CTAs of the first kernel shared:
-// its parts, in order, over the four warps, then the warps.
-template <int DV, int NT>
-__global__ void __launch_bounds__(128) kv4_join_k(const Kv4AttnArgs a) {
+// One CTA a row of an item whose units several CTAs of the first kernel shared: the largest
+// reference of its parts, then their weighted sum, a fixed set of parts a warp, then the warps.
+template <int DV, int NT, int kJoinWarps>
+__global__ void __launch_bounds__(32 * kJoinWarps) kv4_join_k(const Kv4AttnArgs a) {
   constexpr int ROWS = 8 * NT, N = DV / 32;
-  __shared__ float sm[4], sl[4], so[4][DV];
+  __shared__ float sm[kJoinWarps], sl[kJoinWarps], so[kJoinWarps][DV];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int R = a.H / a.Hk * a.Lq, tiles = (R + ROWS - 1) / ROWS, per = a.Hk * tiles;
   const int item = blockIdx.x % per, hk = item / tiles, rr = blockIdx.y, r = (item - hk * tiles) * ROWS + rr;
@@ -758,33 +758,41 @@ __global__ void __launch_bounds__(128) kv4_join_k(const Kv4AttnArgs a) {
   const int u0 = before + item * (kHead + units) + kHead, c0 = u0 / share, c1 = (u0 + units - 1) / share;
   asm volatile("griddepcontrol.wait;" ::: "memory");   // the first kernel is done and its writes are here
   if (r >= R || c0 == c1) return;                      // one CTA had it whole and has written it
-  float acc[N], m = -kUnset, l = 0.f;
+  // where CTA c left it: slot 0, the first item of its share, but for a CTA c0 whose share begins before it (and its
+  // blank units)
+  const int late = c0 * share < u0 - kHead;
+  auto place = [&](int c) { return (2LL * c + (c == c0 ? late : 0)) * ROWS + rr; };
+  float top = -kUnset;
+  for (int c = c0 + threadIdx.x; c <= c1; c += 32 * kJoinWarps) top = fmaxf(top, a.part_ml[2 * place(c)]);
+  top = warp_max(top);
+  if (lane == 0) sm[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, sm[w]);
+  float acc[N], l = 0.f;
 #pragma unroll
   for (int j = 0; j < N; ++j) acc[j] = 0.f;
-  for (int c = c0 + warp; c <= c1; c += 4) {
-    // it is the first item of CTA c0's share where that begins with it (or with its blank units)
-    const long long at = (2LL * c + (c == c0 && c0 * share < u0 - kHead ? 1 : 0)) * ROWS + rr;
+#pragma unroll 4
+  for (int c = c0 + warp; c <= c1; c += kJoinWarps) {
+    const long long at = place(c);
     const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * at);
-    const float to = fmaxf(m, ml.x), keep = ex2_approx(m - to), add = ex2_approx(ml.x - to);
-    m = to;
-    l = l * keep + ml.y * add;
+    const float f = ex2_approx(ml.x - top);
     const float* po = a.part_o + at * DV + N * lane;
+    l += f * ml.y;
 #pragma unroll
-    for (int j = 0; j < N; ++j) acc[j] = acc[j] * keep + po[j] * add;
+    for (int j = 0; j < N; ++j) acc[j] += f * po[j];
   }
-  if (lane == 0) { sm[warp] = m; sl[warp] = l; }
+  if (lane == 0) sl[warp] = l;
 #pragma unroll
   for (int j = 0; j < N; ++j) so[warp][N * lane + j] = acc[j];
   __syncthreads();
   if (threadIdx.x >= DV / 2) return;
-  const float top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
   float sum = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const float c = ex2_approx(sm[w] - top);
-    sum += c * sl[w];
-    x += c * so[w][2 * threadIdx.x];
-    y += c * so[w][2 * threadIdx.x + 1];
+  for (int w = 0; w < kJoinWarps; ++w) {
+    sum += sl[w];
+    x += so[w][2 * threadIdx.x];
+    y += so[w][2 * threadIdx.x + 1];
   }
   store_row<DV>(a, seq, hk, r, 2 * threadIdx.x, sum, x, y);
 }
@@ -875,7 +883,11 @@ int attn_launch(const Kv4AttnArgs& a, cudaStream_t st) {
   // launched while the first kernel runs; it waits for that one's writes itself
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
-  return launch_with(kv4_join_k<DV, NT>, dim3(items, R < 8 * NT ? R : 8 * NT), 128, st, attr, a);
+  const dim3 rows(items, R < 8 * NT ? R : 8 * NT);
+  // eight warps where an item has many parts (131072 tokens of one head: 20 us against 37), four where most have one
+  // or two (1024 items of 300 tokens: 28 us against 33)
+  if (a.ctas > 16LL * items) return launch_with(kv4_join_k<DV, NT, 8>, rows, 256, st, attr, a);
+  return launch_with(kv4_join_k<DV, NT, 4>, rows, 128, st, attr, a);
 }
 
 }  // namespace
