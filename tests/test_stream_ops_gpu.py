@@ -130,6 +130,21 @@ def test_rotary_empty():
         assert yq.shape == (B, L, H, 8) and yk.shape == (B, L, Hk, 8)
 
 
+def test_rotary_wide_heads_and_many_tokens():
+    for B, L, H, Hk, D, R in ((1, 2, 1, 1, 4096, 4096), (300, 7, 1, 0, 8, 2), (5, 4001, 2, 1, 64, 16)):
+        for layout in LAYOUTS:
+            q, k = torch.randn(B, L, H, D, device=DEV), torch.randn(B, L, Hk, D, device=DEV)
+            inv = frequencies(R).to(DEV)
+            yq, yk = ops.rotary(q, k, 3, inv, layout=layout)
+            pos = (3 + torch.arange(L, device=DEV)).expand(B, L)
+            rotary_close(q, yq, pos, inv, layout, 1.0)
+            if Hk:
+                rotary_close(k, yk, pos, inv, layout, 1.0)
+    with pytest.raises(ValueError, match="8192"):
+        x = torch.zeros(1, 1, 1, 8194, device=DEV)
+        ops.rotary(x, None, 0, torch.zeros(4097, device=DEV))
+
+
 # ------------------------------------------------------------------ 4-bit cache --
 
 def plain_cache(k, v, cap, start):
@@ -196,6 +211,16 @@ def test_append_extremes_equal_the_plain_form():
     assert torch.equal(ky.cpu()[~wy.isnan()], wy[~wy.isnan()])
     fine = ~wy.isnan().reshape(40, 64).any(1)
     assert torch.equal(c.k_codes.cpu()[0, 0, :40][fine], want.k_codes[0, 0, :40][fine])
+
+
+def test_append_many_sequences_and_unequal_dims():
+    for B, L, D, Dv in ((70000, 1, 32, 64), (3, 700, 512, 32), (2, 5, 32, 1024)):
+        k, v = torch.randn(B, 1, L, D, device=DEV).bfloat16(), torch.randn(B, 1, L, Dv, device=DEV).bfloat16()
+        c = ops.Int4KV.empty(B, 1, L, D, Dv, device=DEV)
+        ops.int4_append(c, k, v, 0)
+        ky, vy = ops.int4_read(c, 0, L)
+        held_by_the_definition(k, c.k_codes[:, :, :L], c.k_params[:, :, :L], ky)
+        held_by_the_definition(v, c.v_codes[:, :, :L], c.v_params[:, :, :L], vy)
 
 
 def test_append_strides():
@@ -420,6 +445,15 @@ def test_verify_strides():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_verify_many_rows():
+    B = 70000
+    p = torch.rand(B, 1, 3, device=DEV)
+    none, us = torch.zeros(B, 0, device=DEV), torch.rand(B, device=DEV)
+    run = p[:, 0].double().cumsum(-1)
+    want = (run > us.double()[:, None] * run[:, -1:]).int().argmax(1)
+    assert torch.equal(ops.verify_draft(p, None, none.long(), none, us)[0][:, 0], want)
+
+
 def test_verify_empty_batch():
     out, acc = ops.verify_draft(torch.empty(0, 4, 10, device=DEV), None, torch.empty(0, 3, device=DEV).long(),
                                 torch.empty(0, 3, device=DEV), torch.empty(0, device=DEV))
@@ -499,6 +533,50 @@ def test_together_on_a_side_stream_and_in_a_graph():
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(out, expect))
+
+
+def test_two_streams_at_once():
+    """Attention and verification on two streams whose work overlaps; each has its own scratch."""
+    a, b = _chain_inputs(2), _chain_inputs(3)
+    big = filled(2, 4, 20000, 128, 128)
+    q = torch.randn(2, 8, 1, 128, device=DEV).bfloat16()
+    want = [_chain(**a), _chain(**b), ops.int4_attention(q, big, 20000)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = [None] * 3
+    for _ in range(5):
+        for i, run in enumerate((lambda: _chain(**a), lambda: _chain(**b), lambda: ops.int4_attention(q, big, 20000))):
+            with torch.cuda.stream(streams[i]):
+                got[i] = run()
+    torch.cuda.synchronize()
+    for x, y in zip(got[0] + got[1] + (got[2],), want[0] + want[1] + (want[2],)):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("B,H,Hk,Lq,T,D", [(1, 4, 4, 200, 700, 128), (2, 4, 2, 150, 3000, 64), (1, 2, 2, 130, 130, 64)])
+def test_attention_many_queries(B, H, Hk, Lq, T, D):
+    """Long blocks of queries, which may be served from unpacked values, and the same with lengths on the GPU."""
+    c = filled(B, Hk, T, D, D)
+    q = (2 * torch.randn(B, H, Lq, D, device=DEV)).bfloat16()
+    n = torch.full((B,), T, device=DEV)
+    for causal in (True, False):
+        attention_close(q, c, n, ops.int4_attention(q, c, T, causal=causal), causal)
+        attention_close(q, c, n, ops.int4_attention(q, c, n, causal=causal), causal)
+
+
+def test_attention_unpacked_first_equals_the_kernel():
+    """Enough queries over enough tokens that the values are unpacked first (two orders of summation of one result)."""
+    c = filled(1, 8, 4096, 128, 128)
+    q = torch.randn(1, 8, 1024, 128, device=DEV).bfloat16()
+    a = ops.int4_attention(q, c, 4096).double()
+    b = ops.int4_attention(q, c, torch.full((1,), 4096, device=DEV)).double()
+    k, v = ops.int4_read(c, 0, 4096)
+    s = (q.double() @ k.double().transpose(-1, -2) / 128 ** 0.5)
+    s = s.masked_fill(torch.ones(1024, 4096, dtype=torch.bool, device=DEV).triu(4096 - 1024 + 1), float("-inf"))
+    p = torch.softmax(s, -1)
+    want, mag = p @ v.double(), p @ v.double().abs()
+    for x in (a, b):      # output and probabilities to bf16, scores as in attention_close, the exponential's fit to 7.5e-5
+        assert ((x - want).abs() <= 2 ** -8 * want.abs() + (2 ** -8 + 2e-4 + 2 ** -9) * mag).all()
 
 
 def test_rotary_backward_in_a_graph():

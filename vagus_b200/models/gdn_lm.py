@@ -85,6 +85,9 @@ class GDNLM(CausalLM):
             self.rope = RoPE(dim, softmax_head_dim, context_len, base=rope_base, rotary_dim=rope_dim,
                              layout=rope_layout, scaling=rope_scaling)
 
+        assert self.rope is not None or not rope_options(rope_dim, rope_layout, rope_scaling), \
+            "rope options without a rotary softmax layer"
+
         assert write in WRITES, f"write must be one of {WRITES}, got {write!r}"
         self.write = write
 

@@ -37,7 +37,7 @@ def rope_frequencies(rotary_dim: int, base: float, scaling: dict | None = None) 
     fewer than beta_slow times over the original length, keeps those that turn
     more than beta_fast times, blends between, and multiplies q and k by
     0.1 ln f + 1."""
-    i = torch.arange(rotary_dim // 2, dtype=torch.float64)
+    i = torch.arange(rotary_dim // 2, dtype=torch.float64, device="cpu")
     inv = float(base) ** (-2 * i / rotary_dim)
     if scaling is None:
         return inv, 1.0

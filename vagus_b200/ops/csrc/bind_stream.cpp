@@ -98,6 +98,7 @@ std::tuple<Tensor, OptTensor> rotary(Tensor q, OptTensor k, OptTensor pos, int64
   TORCH_CHECK_VALUE(inv.dim() == 1 && inv.is_floating_point() && inv.size(0) >= 1 && inv.size(0) <= a.D / 2 &&
                         inv.device() == q.device(),
                     "rotary: inv_freq (R/2,) on q's device with 2 <= R <= " + str(a.D));
+  TORCH_CHECK_VALUE(inv.size(0) <= 4096, "rotary: R up to 8192 on the GPU");
   if (inv.scalar_type() != at::kDouble) inv = inv.to(at::kDouble);
   inv = inv.contiguous();
   a.inv = inv.data_ptr<double>();
@@ -130,8 +131,9 @@ Cache cache_of(const Tensor& kc, const Tensor& kp, const Tensor& vc, const Tenso
   TORCH_CHECK_VALUE(c.D > 0 && c.Dv > 0 && c.D % 32 == 0 && c.Dv % 32 == 0 && kp.size(3) == c.D / 32 &&
                         vp.size(3) == c.Dv / 32 && kp.size(4) == 2 && vp.size(4) == 2,
                     "Int4KV: head dims in groups of 32 with two parameters each");
-  TORCH_CHECK_VALUE(c.cap % 16 == 0 && c.cap < (int64_t(1) << 31) - 64,
-                    "Int4KV: the capacity must be a multiple of 16");
+  TORCH_CHECK_VALUE(c.D <= 4096 && c.Dv <= 4096, "Int4KV: head dims up to 4096 on the GPU");
+  TORCH_CHECK_VALUE(c.cap % 16 == 0 && c.cap < (int64_t(1) << 30),
+                    "Int4KV: the capacity must be a multiple of 16, below 2^30");
   return c;
 }
 
@@ -301,7 +303,11 @@ std::tuple<Tensor, Tensor> verify_draft(Tensor target, OptTensor draft, Tensor t
 
 void register_stream_ops(pybind11::module& m) {
   m.def("rotary", &rotary);
-  m.def("kv4_check", [](Tensor kc, Tensor kp, Tensor vc, Tensor vp) { cache_of(kc, kp, vc, vp); });
+  m.def("kv4_check", [](Tensor kc, Tensor kp, Tensor vc, Tensor vp) {
+    cache_of(kc, kp, vc, vp);
+    c10::cuda::CUDAGuard guard(kc.device());
+    vagus_device_error_ptr();             // made here, so that the first use may be captured into a graph
+  });
   m.def("kv4_append", &kv4_append);
   m.def("kv4_read", &kv4_read);
   m.def("kv4_attn", &kv4_attn);

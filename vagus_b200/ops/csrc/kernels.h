@@ -217,9 +217,10 @@ struct Kv4AppendArgs {
   void *k_codes, *k_params, *v_codes, *v_params;
   const void* start; int start_i64; long long offset;       // per sequence, or null: offset
   long long B, L, cap; int Hk, D, Dv;
+  unsigned blocks;                              // blocks of a sequence: set by kv4_append
   int* err;
 };
-int kv4_append(const Kv4AppendArgs& a, int type, cudaStream_t st);
+int kv4_append(Kv4AppendArgs a, int type, cudaStream_t st);
 struct Kv4ReadArgs {
   const void *k_codes, *k_params, *v_codes, *v_params;
   void *k, *v;                                  // (B, Hk, L, D | Dv) bf16 dense
@@ -257,6 +258,7 @@ struct VerifyArgs {
   long long* out;                               // (B, K + 1)
   long long* accepted;                          // (B)
   long long B, V; int K;
+  int cluster;                                  // set by verify_draft
 };
 int verify_draft(const VerifyArgs& a, int type, cudaStream_t st);
 

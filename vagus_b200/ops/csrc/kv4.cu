@@ -106,13 +106,17 @@ __device__ __forceinline__ float fifteenth(float x) {
 // reads and writes alone would take 54), with every issue slot in three used.
 template <typename T, bool VEC, int ROWS>
 __global__ void __launch_bounds__(256) kv4_append_k(const Kv4AppendArgs a) {
-  const int which = blockIdx.z;                       // 0: keys, 1: values
+  const int which = blockIdx.y;                       // 0: keys, 1: values
   const int D = which ? a.Dv : a.D, per = D / 16, rows = 256 / per;
   const int ty = threadIdx.x / per, part = threadIdx.x - ty * per;
-  const long long b = blockIdx.y;
+  const unsigned seq = blockIdx.x / a.blocks, block = blockIdx.x - seq * a.blocks;
+  const long long b = seq;
   const T* x = static_cast<const T*>(which ? a.v : a.k) + b * (which ? a.sv_b : a.sk_b) + 16 * part;
   const long long sh = which ? a.sv_h : a.sk_h, sl = which ? a.sv_l : a.sk_l;
-  const unsigned total = static_cast<unsigned>(a.L) * a.Hk, Hk = a.Hk, r0 = blockIdx.x * (rows * ROWS) + ty;
+  const unsigned total = static_cast<unsigned>(a.L) * a.Hk, Hk = a.Hk;
+  const unsigned long long begin = static_cast<unsigned long long>(block) * (rows * ROWS);
+  if (begin >= total) return;                         // the narrower of keys and values takes fewer blocks
+  const unsigned r0 = static_cast<unsigned>(begin) + ty;
   const long long start = a.start ? index_at(a.start, a.start_i64, b) : a.offset;
   const bool idle = ty >= rows;                       // threads past the last whole row of threads
 
@@ -892,15 +896,17 @@ int attn_launch(const Kv4AttnArgs& a, cudaStream_t st) {
 
 }  // namespace
 
-int kv4_append(const Kv4AppendArgs& a, int type, cudaStream_t st) {
+int kv4_append(Kv4AppendArgs a, int type, cudaStream_t st) {
   if (a.D % kGroup || a.Dv % kGroup || a.D < kGroup || a.Dv < kGroup || a.D > 4096 || a.Dv > 4096) return 1;
   if (a.B * a.L * a.Hk == 0) return 0;
   const int widest = a.D > a.Dv ? a.D : a.Dv, rows = 256 / (widest / 16);     // rows a block takes at once
-  if (a.L * a.Hk > 0x7fffffffLL - 4096 || a.B > 65535) return 2;
+  if (a.L * a.Hk > 0x7fffffffLL - 65536) return 2;
   // four rows a thread, whose loads overlap, once that still makes several blocks an SM; one row below (300 tokens
   // of 16 heads of 64: 2.6 us against 4.1)
   const int each = a.B * ((a.L * a.Hk + 4 * rows - 1) / (4 * rows)) >= 148 * 4 ? 4 : 1;
-  const dim3 grid(static_cast<unsigned>((a.L * a.Hk + each * rows - 1) / (each * rows)), static_cast<unsigned>(a.B), 2);
+  a.blocks = static_cast<unsigned>((a.L * a.Hk + each * rows - 1) / (each * rows));
+  if (a.B * a.blocks > 0x7fffffffLL) return 2;
+  const dim3 grid(static_cast<unsigned>(a.B * a.blocks), 2);
   const int es = type == 0 ? 4 : 2;
   auto al = [es](const void* p, long long x, long long y, long long z) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && x * es % 16 == 0 && y * es % 16 == 0 && z * es % 16 == 0;

@@ -37,7 +37,7 @@ struct alignas(16) Vec {
 };
 
 constexpr int kThreads = 256;
-constexpr int kMaxAngles = 1024;     // pairs of angles of a CTA's tokens in shared memory
+constexpr int kMaxAngles = 4096;     // pairs of angles of a CTA's tokens in shared memory
 
 __device__ __forceinline__ long long position_of(const RotaryArgs& a, long long b, long long l) {
   if (a.pos == nullptr) return a.offset + l;
@@ -184,6 +184,7 @@ int launch(const RotaryArgs& a, cudaStream_t st) {
   // tokens a CTA: as many as its threads have angles for at once, fewer while the grid would not fill the GPU
   int tokens = half >= kThreads ? 1 : kThreads / half;
   while (tokens > 1 && (a.B * a.L + tokens - 1) / tokens < 148 * 4) --tokens;
+  while (tokens > 1 && static_cast<long long>(tokens) * (a.H + a.Hk) * a.D > 1 << 30) --tokens;
   const long long grid = (a.B * a.L + tokens - 1) / tokens;
   if (a.B * a.L > 0x7fff0000LL) return 2;                // tokens are counted in 32 bits
   const size_t smem = static_cast<size_t>(tokens) * half * sizeof(float2);

@@ -120,8 +120,9 @@ __global__ void __launch_bounds__(kThreads, 4) verify_k(const VerifyArgs a) {
   __shared__ double cta_total;
   __shared__ int s_acc;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int rank = blockIdx.x, C = gridDim.x;          // the cluster spans grid.x
-  const long long b = blockIdx.y;
+  const int C = a.cluster;                             // CTAs of a row, which are a cluster
+  const long long b = blockIdx.x / C;
+  const int rank = static_cast<int>(blockIdx.x - b * C);
   const T* target = static_cast<const T*>(a.target) + b * a.st_b;
   const T* draft = a.draft ? static_cast<const T*>(a.draft) + b * a.sd_b : nullptr;
   const long long* tok = a.tokens + b * a.stok_b;
@@ -265,7 +266,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_k(const VerifyArgs a) {
 }
 
 template <typename T>
-int launch(const VerifyArgs& a, cudaStream_t st) {
+int launch(VerifyArgs a, cudaStream_t st) {
   // CTAs a row: enough to fill the GPU, each with 1024 candidates at least
   int C = 1;
   while (C < kMaxCluster && a.B * C < 148 * 2 && a.V > static_cast<long long>(C) * 1024) C *= 2;
@@ -273,7 +274,8 @@ int launch(const VerifyArgs& a, cudaStream_t st) {
   const bool vec = al(a.target) && a.V % 4 == 0 && a.st_b % 4 == 0 && a.st_k % 4 == 0 &&
                    (!a.draft || (al(a.draft) && a.sd_b % 4 == 0 && a.sd_k % 4 == 0));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(C, static_cast<unsigned>(a.B));
+  a.cluster = C;
+  cfg.gridDim = dim3(static_cast<unsigned>(a.B * C));
   cfg.blockDim = dim3(kThreads);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -290,7 +292,8 @@ int launch(const VerifyArgs& a, cudaStream_t st) {
 }  // namespace
 
 int verify_draft(const VerifyArgs& a, int type, cudaStream_t st) {
-  if (a.V < 1 || a.K < 0 || a.B > 65535) return 1;
+  if (a.V < 1 || a.K < 0) return 1;
+  if (a.B > 0x0fffffffLL) return 2;
   if (a.B == 0) return 0;
   if (type == 0) return launch<float>(a, st);
   if (type == 1) return launch<__half>(a, st);

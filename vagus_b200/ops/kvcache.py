@@ -39,8 +39,8 @@ def _check_cache(k_codes, k_params, v_codes, v_params) -> None:
             raise ValueError(f"Int4KV: {what}_params must be {want} bf16, contiguous")
     if k_codes.shape[:3] != v_codes.shape[:3]:
         raise ValueError("Int4KV: keys and values must agree in batch, heads and capacity")
-    if k_codes.shape[2] % _BLOCK:
-        raise ValueError(f"Int4KV: the capacity must be a multiple of {_BLOCK}")
+    if k_codes.shape[2] % _BLOCK or k_codes.shape[2] >= 1 << 30:
+        raise ValueError(f"Int4KV: the capacity must be a multiple of {_BLOCK}, below 2^30")
     if any(t.device != k_codes.device for t in (k_params, v_codes, v_params)):
         raise ValueError("Int4KV: the tensors must be on one device")
 
@@ -231,9 +231,11 @@ def int4_attention(q, cache: Int4KV, lengths, causal: bool = True):
     clamps it to the cache and reports it through ``check_error``).  With
     ``causal`` the queries are the last Lq of those tokens: query i sees the
     first lengths - Lq + i + 1 of them.  A query that sees nothing gives zeros.
-    What the cache holds past a sequence's length has no effect.  Inference
-    only: no gradient flows.  The kernels take bf16 queries and head dims 64 and
-    128; the plain form serves the others."""
+    What the cache holds past a sequence's length has no effect; a NaN inside it
+    may reach every query of the call.  Inference only: no gradient flows.  The
+    kernels take bf16 queries and head dims 64 and 128, the plain form serves the
+    others; with many queries over equal lengths (an int) the values are unpacked
+    into a temporary bf16 copy first."""
     per, at = _place(lengths, "int4_attention: lengths")
     if cache.k_codes.is_cuda:
         o = native().kv4_attn(q, cache.k_codes, cache.k_params, cache.v_codes, cache.v_params, per, at, causal)
