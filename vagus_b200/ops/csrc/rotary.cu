@@ -71,9 +71,10 @@ __device__ __forceinline__ void row_of(const RotaryArgs& a, long long b, long lo
 // layout's rotated channels the two vectors that pair up.  The angles of an item's P pairs
 // are read as float4s of two; those lie [which of the P / 2][item], so that neighbouring
 // threads read neighbouring 16 bytes (item-major, 8 threads met in 2 of 8 bank groups).
-// Many resident threads matter more than loads held ahead in registers: two to four rows'
-// loads first took 146 to 187 us instead of 99 for both directions of 4 x 4096 tokens of 32
-// heads of 128 in bf16 (5.3 TB/s; fp32 6.2 TB/s).
+// A head's address is worked out once and its tokens follow.  Many resident threads matter
+// more than loads held ahead in registers (rows' loads taken two to four at a time: 146 to
+// 187 us for both directions of 4 x 4096 tokens of 32 heads of 128 in bf16, 105 so: 5.0
+// TB/s, and 6.2 TB/s in fp32, which has half the arithmetic a byte).
 template <typename T, bool INTER>
 __global__ void __launch_bounds__(kThreads, INTER ? 8 : 6) rotary_vec_k(const RotaryArgs a, int tokens, int across) {
   constexpr int N = Vec<T>::N, P = INTER ? N / 2 : N;
@@ -105,7 +106,7 @@ __global__ void __launch_bounds__(kThreads, INTER ? 8 : 6) rotary_vec_k(const Ro
     const long long* at = is_q ? q_at : k_at;
     const long long pitch = static_cast<long long>(is_q ? a.H : a.Hk) * a.D;
     T* out = (is_q ? static_cast<T*>(a.yq) + h * a.D : static_cast<T*>(a.yk) + (h - a.H) * a.D) + t0 * pitch;
-#pragma unroll 2
+#pragma unroll 1
     for (int tk = ty; tk < nt; tk += tstep) {
       const float4* c = reinterpret_cast<const float4*>(cs + tk * half) + item;
       const T* src = in + at[tk] + c0;
