@@ -130,6 +130,12 @@ def test_rotary_empty():
         assert yq.shape == (B, L, H, 8) and yk.shape == (B, L, Hk, 8)
 
 
+def test_rotary_refuses_a_token_past_32_bits():
+    q = torch.zeros(1, 1, 1, 2, device=DEV).bfloat16().expand(1, 1, 1 << 30, 2)
+    with pytest.raises(RuntimeError, match="rejected"):
+        ops.rotary(q, None, 0, frequencies(2).to(DEV))
+
+
 def test_rotary_wide_heads_and_many_tokens():
     for B, L, H, Hk, D, R in ((1, 2, 1, 1, 4096, 4096), (300, 7, 1, 0, 8, 2), (5, 4001, 2, 1, 64, 16)):
         for layout in LAYOUTS:
@@ -253,6 +259,30 @@ def test_append_outside_is_reported_and_writes_nothing():
     assert (y[0, :, 1] == 0).all() and (y[1, :, 0] == 0).all() and (y[2] != 0).any(-1).all()
 
 
+def test_places_at_the_ends_of_64_bits():
+    """Places whose sums with a token's index leave 64 bits are outside like any other."""
+    far = torch.tensor([2 ** 63 - 1, -2 ** 63, 2 ** 60, -2 ** 60, 2 ** 62 - 1, 3], device=DEV)
+    for L in (2, 300):
+        c = ops.Int4KV.empty(6, 1, 320, 64, device=DEV)
+        x = torch.randn(6, 1, 320, 64, device=DEV)
+        ops.int4_append(c, x, x, 0)
+        before = [t.clone() for t in c.tensors()]
+        ops.int4_append(c, x[:, :, :L].flip(2).contiguous(), x[:, :, :L], far)
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="outside"):
+            ops.check_error()
+        assert all(torch.equal(t[:5], u[:5]) for t, u in zip(c.tensors(), before))
+        y, _ = ops.int4_read(c, far, L)
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="outside"):
+            ops.check_error()
+        assert (y[:5] == 0).all() and torch.equal(y[5], ops.int4_read(c, 3, L)[0][5])
+        for call in (lambda: ops.int4_append(c, x[:, :, :L], x[:, :, :L], 2 ** 63 - 1),
+                     lambda: ops.int4_read(c, 2 ** 63 - 1, L), lambda: ops.int4_read(c, 0, 2 ** 63 - 1)):
+            with pytest.raises(ValueError):
+                call()
+
+
 # -------------------------------------------------------------------- attention --
 
 def filled(B, Hk, cap, D, Dv):
@@ -327,6 +357,17 @@ def test_attention_large_scores_and_one_key():
     q = (40 * k[:, :, 37:38].float()).bfloat16()
     got = ops.int4_attention(q, c, 96, causal=False)
     assert torch.equal(got, v[:, :, 37:38])
+
+
+def test_attention_scores_far_below_zero():
+    """Scores of -1e35 and less: the nearest key still takes all the weight."""
+    c = ops.Int4KV.empty(1, 1, 32, 64, device=DEV)
+    k = -1e16 * torch.arange(1, 21, device=DEV).float()[:, None].expand(1, 1, 20, 64)
+    ops.int4_append(c, k.contiguous(), torch.randn(1, 1, 20, 64, device=DEV), 0)
+    q = torch.full((1, 2, 1, 64), 1e18, device=DEV).bfloat16()
+    v = ops.int4_read(c, 0, 20)[1]
+    for lengths in (20, torch.tensor([20], device=DEV), 1):
+        assert torch.equal(ops.int4_attention(q, c, lengths), v[:, :, :1].expand(1, 2, 1, 64))
 
 
 def test_attention_strided_queries_and_other_types():
@@ -577,6 +618,25 @@ def test_attention_unpacked_first_equals_the_kernel():
     want, mag = p @ v.double(), p @ v.double().abs()
     for x in (a, b):      # output and probabilities to bf16, scores as in attention_close, the exponential's fit to 7.5e-5
         assert ((x - want).abs() <= 2 ** -8 * want.abs() + (2 ** -8 + 2e-4 + 2 ** -9) * mag).all()
+
+
+def test_attention_broadcast_queries_unpacked_first():
+    c = filled(1, 8, 4096, 128, 128)
+    q = torch.randn(1, 1, 1, 128, device=DEV).bfloat16().expand(1, 8, 1024, 128)
+    assert torch.equal(ops.int4_attention(q, c, 4096), ops.int4_attention(q.contiguous(), c, 4096))
+
+
+def test_rope_frequencies_first_used_in_inference_mode():
+    from vagus_b200.models.rope import RoPE
+    rope = RoPE(64, 64, 32, layout="half").to(DEV)
+    x = torch.randn(1, 5, 1, 64, device=DEV)
+    with torch.inference_mode():
+        y = rope.rotate(x, None)
+    x.requires_grad_()
+    z = rope.rotate(x, None)
+    assert torch.equal(y, z.detach())
+    z.square().sum().backward()                   # a rotation keeps the length: the gradient of its square is 2 x
+    assert (x.grad - 2 * x).abs().max() <= 2 * 2 * 8e-7 * 2 * x.detach().abs().max()
 
 
 def test_rotary_backward_in_a_graph():

@@ -107,7 +107,8 @@ class RoPE(nn.Module):
         """Angle per step of position, float64 whatever the module was cast to."""
         device = torch.device(device)
         if device not in self._inv_on:
-            self._inv_on[device] = self._inv.to(device)
+            with torch.inference_mode(False):          # kept past the call: training may save it for its backward
+                self._inv_on[device] = self._inv.to(device)
         return self._inv_on[device]
 
     def prepare_m(self, L: int) -> None:

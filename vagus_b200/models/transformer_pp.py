@@ -26,7 +26,8 @@ class TransformerPP(CausalLM):
         self.config: dict[str, Any] = dict(
             vocab_size=vocab_size, dim=dim, head_dim=head_dim, context_len=context_len,
             layer_count=layer_count, ffn_hidden_dim=ffn_hidden_dim, kv_head_count=kv_head_count,
-            rmsnorm_eps=rmsnorm_eps, rope_base=rope_base, tie_embedding=tie_embedding, qk_norm=qk_norm, **rope_options(rope_dim, rope_layout, rope_scaling))
+            rmsnorm_eps=rmsnorm_eps, rope_base=rope_base, tie_embedding=tie_embedding, qk_norm=qk_norm,
+            **rope_options(rope_dim, rope_layout, rope_scaling))
         assert dim % head_dim == 0
         self.embedding = nn.Embedding(vocab_size, dim)
         self.rope = RoPE(dim, head_dim, context_len, base=rope_base, rotary_dim=rope_dim, layout=rope_layout,

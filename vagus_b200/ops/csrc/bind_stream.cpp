@@ -165,8 +165,8 @@ void kv4_append(Tensor kc, Tensor kp, Tensor vc, Tensor vp, Tensor k, Tensor v, 
   a.sv_b = v.stride(0); a.sv_h = v.stride(1); a.sv_l = v.stride(2);
   a.k_codes = kc.data_ptr(); a.k_params = kp.data_ptr(); a.v_codes = vc.data_ptr(); a.v_params = vp.data_ptr();
   per_row(start, c, a.start, a.start_i64, "int4_append: start");
-  TORCH_CHECK_VALUE(a.start || (offset >= 0 && offset + L <= c.cap), "int4_append: tokens [" + str(offset) + ", " +
-                    str(offset + L) + ") leave the cache of " + str(c.cap));
+  TORCH_CHECK_VALUE(a.start || (offset >= 0 && L <= c.cap && offset <= c.cap - L), "int4_append: " + str(L) +
+                    " tokens from " + str(offset) + " on leave the cache of " + str(c.cap));
   a.offset = offset;
   a.B = c.B; a.L = L; a.cap = c.cap; a.Hk = static_cast<int>(c.Hk); a.D = static_cast<int>(c.D);
   a.Dv = static_cast<int>(c.Dv);
@@ -180,8 +180,8 @@ std::tuple<Tensor, Tensor> kv4_read(Tensor kc, Tensor kp, Tensor vc, Tensor vp, 
   c10::cuda::CUDAGuard guard(kc.device());
   vagus::Kv4ReadArgs a = {};
   per_row(start, c, a.start, a.start_i64, "int4_read: start");
-  TORCH_CHECK_VALUE(count >= 0 && (a.start || (offset >= 0 && offset + count <= c.cap)), "int4_read: tokens [" +
-                    str(offset) + ", " + str(offset + count) + ") leave the cache of " + str(c.cap));
+  TORCH_CHECK_VALUE(count >= 0 && (a.start || (offset >= 0 && count <= c.cap && offset <= c.cap - count)), "int4_read: " +
+                    str(count) + " tokens from " + str(offset) + " on leave the cache of " + str(c.cap));
   auto k = fresh({c.B, c.Hk, count, c.D}, at::kBFloat16, kc), v = fresh({c.B, c.Hk, count, c.Dv}, at::kBFloat16, kc);
   a.k_codes = kc.data_ptr(); a.k_params = kp.data_ptr(); a.v_codes = vc.data_ptr(); a.v_params = vp.data_ptr();
   a.k = k.data_ptr(); a.v = v.data_ptr();
@@ -209,7 +209,7 @@ c10::optional<Tensor> kv4_attn(Tensor q, Tensor kc, Tensor kp, Tensor vc, Tensor
   if (q.scalar_type() != at::kBFloat16 || (c.D != 64 && c.D != 128) || (c.Dv != 64 && c.Dv != 128))
     return c10::nullopt;
   bool ok = q.stride(3) == 1 && reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0;
-  for (int d = 0; d < 3; ++d) ok = ok && q.stride(d) % 8 == 0;
+  for (int d = 0; d < 3; ++d) ok = ok && q.stride(d) > 0 && q.stride(d) % 8 == 0;       // tensor maps take no stride of zero
   if (!ok) q = q.clone(at::MemoryFormat::Contiguous);
   a.q = q.data_ptr();
   a.sq_b = q.stride(0); a.sq_h = q.stride(1); a.sq_l = q.stride(2);

@@ -171,8 +171,8 @@ __global__ void __launch_bounds__(256) kv4_append_k(const Kv4AppendArgs a) {
     lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, 1));
     hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, 1));
     if (!live) continue;
-    const long long t = start + l;
-    if (t < 0 || t >= a.cap) {                        // a start given on the device that leaves the cache
+    const unsigned long long t = static_cast<unsigned long long>(start) + l;
+    if (t >= static_cast<unsigned long long>(a.cap)) {        // a start given on the device that leaves the cache
       record_error(a.err, kErrBadArgument);
       continue;
     }
@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(256) kv4_append_k(const Kv4AppendArgs a) {
     const float s = __bfloat162float(s16);
     const __nv_bfloat16 b16 = __float2bfloat16_rn(__fsub_rn(lo, __fmul_rn(128.f, s)));
     const uint2 w = codes_of(v, s, __bfloat162float(b16));
-    const long long out = (b * a.Hk + h) * a.cap + t;
+    const long long out = (b * a.Hk + h) * a.cap + static_cast<long long>(t);
     reinterpret_cast<uint2*>(which ? a.v_codes : a.k_codes)[out * per + part] = w;
     if ((part & 1) == 0) {
       const __nv_bfloat162 pr = __halves2bfloat162(s16, b16);
@@ -226,7 +226,9 @@ __global__ void __launch_bounds__(256) kv4_read_k(const Kv4ReadArgs a, unsigned 
   const unsigned per_head = static_cast<unsigned>((words + 256 * kReadWords - 1) / (256 * kReadWords));
   const unsigned bh = block / per_head;
   const long long i0 = static_cast<long long>(block - bh * per_head) * (256 * kReadWords) + threadIdx.x;
-  const long long start = a.start ? index_at(a.start, a.start_i64, bh / a.Hk) : a.offset;
+  // any start given on the device, brought to where nothing below overflows
+  const long long given = a.start ? index_at(a.start, a.start_i64, bh / a.Hk) : a.offset;
+  const long long start = given < -a.L ? -a.L : given > a.cap ? a.cap : given;
   const long long at = static_cast<long long>(bh) * a.cap + start;
   const uint32_t* codes = reinterpret_cast<const uint32_t*>(which ? a.v_codes : a.k_codes) + at * (D / 8);
   const uint32_t* params = reinterpret_cast<const uint32_t*>(which ? a.v_params : a.k_params) + at * (D / kGroup);
@@ -256,12 +258,12 @@ __global__ void __launch_bounds__(256) kv4_read_few_k(const Kv4ReadArgs a) {
   const unsigned words = static_cast<unsigned>(a.L) * (D / 8), i = blockIdx.x * 256 + threadIdx.x, bh = i / words;
   if (bh >= a.B * a.Hk) return;
   const unsigned iw = i - bh * words, l = iw / (D / 8);
-  const long long t = l + (a.start ? index_at(a.start, a.start_i64, bh / a.Hk) : a.offset);
+  const unsigned long long t = l + static_cast<unsigned long long>(a.start ? index_at(a.start, a.start_i64, bh / a.Hk) : a.offset);
   uint4 x = make_uint4(0, 0, 0, 0);
-  if (t < 0 || t >= a.cap) {
+  if (t >= static_cast<unsigned long long>(a.cap)) {
     record_error(a.err, kErrBadArgument);
   } else {
-    const long long at = (bh * a.cap + t) * (D / 8) + (iw - l * (D / 8));
+    const long long at = (bh * a.cap + static_cast<long long>(t)) * (D / 8) + (iw - l * (D / 8));
     x = unpack(reinterpret_cast<const uint32_t*>(which ? a.v_codes : a.k_codes)[at],
                reinterpret_cast<const uint32_t*>(which ? a.v_params : a.k_params)[at / 4], a.magic);
   }
@@ -315,7 +317,7 @@ constexpr int kAttnWarps = 4;
 constexpr int kUnit = 32 * kAttnWarps;      // tokens
 constexpr int kMaxCluster = 8;
 constexpr int kHead = 2;                    // what starting and ending an item costs, in units
-constexpr float kUnset = 1e30f;             // minus the softmax reference before the first score
+constexpr float kUnset = 3e38f;             // minus the softmax reference before the first score: above any score's
 constexpr float kLazy = 8.f;                // raise the reference when a score exceeds it by so many powers of 2
 
 __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
@@ -474,7 +476,7 @@ struct Running {
   }
 
   // raises the references to the largest scores of this tile where those are above
-  __device__ __forceinline__ void raise(const float (&s)[NT][4], float scale) {
+  __device__ __forceinline__ void raise(const float (&s)[NT][4]) {
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -482,7 +484,7 @@ struct Running {
         float mx = fmaxf(s[j][e], s[j][e + 2]);
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-        const float to = fminf(nref[j][e], -mx * scale), c = ex2_approx(to - nref[j][e]);
+        const float to = fminf(nref[j][e], -mx), c = ex2_approx(to - nref[j][e]);
         nref[j][e] = to;
         l[j][e] *= c;
 #pragma unroll
@@ -493,19 +495,24 @@ struct Running {
       }
   }
 
-  // scores -> probabilities against the references, added to the sums; as B operands in p
+  // scores -> probabilities against the references, added to the sums; as B operands in p.  A score is scaled
+  // and rounded before the reference comes off, so that the largest one's power is exactly 0: one fma would
+  // leave the reference's own rounding, which is past 2^127 for scores of 2^31.
   __device__ __forceinline__ void weigh(float (&s)[NT][4], float scale, uint32_t (&p)[NT][2]) {
     float above = -INFINITY;
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) above = fmaxf(above, fmaf(s[j][e], scale, nref[j][e & 1]));
-    if (__any_sync(0xffffffffu, above > kLazy)) raise(s, scale);
+      for (int e = 0; e < 4; ++e) {
+        s[j][e] = __fmul_rn(s[j][e], scale);
+        above = fmaxf(above, s[j][e] + nref[j][e & 1]);
+      }
+    if (__any_sync(0xffffffffu, above > kLazy)) raise(s);
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[j][e] = ex2_approx(fmaf(s[j][e], scale, nref[j][e & 1]));
+        s[j][e] = ex2_approx(s[j][e] + nref[j][e & 1]);
         l[j][e & 1] += s[j][e];
       }
       p[j][0] = transpose8(pack_bf16x2(s[j][0], s[j][1]));
@@ -973,7 +980,7 @@ int kv4_attn_plan(Kv4AttnArgs& a, long long most_tokens) {
 // heads of 128 over 8192 tokens: 55 / 177 / 341 us against 109 / 109 / 111 at 128 / 512 / 1024 rows; over 32768
 // tokens of 16 heads of 64: 103 / 377 / 741 against 381 / 383 / 385.
 bool kv4_attn_unpack_first(const Kv4AttnArgs& a) {
-  if (a.lengths || a.Lq < 128 || a.length < 128 || a.Lq > a.length || a.D != a.Dv) return false;
+  if (a.lengths || a.Lq < 128 || a.length < 128 || a.Lq > a.length || a.D != a.Dv || a.B * a.H == 0) return false;
   const double tiles = (static_cast<double>(a.H / a.Hk) * a.Lq + 15) / 16, units = (a.length + kUnit - 1) / kUnit;
   const double here = 0.0052 * a.B * a.Hk * tiles * units;
   const long long ctas = a.B * a.H * ((a.Lq + 127) / 128), wave = a.D == 64 ? 296 : 148;

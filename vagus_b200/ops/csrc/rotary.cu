@@ -187,7 +187,8 @@ int launch(const RotaryArgs& a, cudaStream_t st) {
   while (tokens > 1 && (a.B * a.L + tokens - 1) / tokens < 148 * 4) --tokens;
   while (tokens > 1 && static_cast<long long>(tokens) * (a.H + a.Hk) * a.D > 1 << 30) --tokens;
   const long long grid = (a.B * a.L + tokens - 1) / tokens;
-  if (a.B * a.L > 0x7fff0000LL) return 2;                // tokens are counted in 32 bits
+  if (a.B * a.L > 0x7fff0000LL) return 2;                // tokens are counted in 32 bits, and so is what one of them holds
+  if (static_cast<long long>(a.H + a.Hk) * a.D > 1 << 30) return 2;
   const size_t smem = static_cast<size_t>(tokens) * half * sizeof(float2);
   auto al = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
   auto mul = [](long long s) { return s % N == 0; };
