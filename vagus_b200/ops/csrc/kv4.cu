@@ -59,15 +59,39 @@ __device__ __noinline__ uint2 codes_by_division(const float* x, float s, float b
   return make_uint2(w[0], w[1]);
 }
 
-// The same in full-rate operations, nine a channel.  q0 = d r with the correctly rounded
-// reciprocal r of s, corrected once by its exact remainder, is the correctly rounded d / s
-// (Markstein); outside the range of s where neither over- nor underflows, by division.
-// (Checking d r for being near to a half and dividing only then took a branch in two warps
-// out of three, since a bf16 x lies exactly half way in one case of 500: 254 us against
-// 115 for 4 x 8191 tokens of 16 heads.)  Adding and subtracting 1.5 * 2^23 rounds to a whole
-// number, ties to even; four codes are gathered as one float, whose low 16 bits they are
-// once 2^23 is added.
-__device__ __forceinline__ uint2 codes_of(const float (&x)[16], float s, float b) {
+// Two floats an operation.
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 pair2(float a, float b) {
+  F2 d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ void halves(F2 x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+
+// The same in operations on two channels at once where there is one (the scalar ones made
+// the append 107 us instead of 91).  q0 = d r with the correctly rounded reciprocal r of s,
+// corrected once by its exact remainder, is the correctly rounded d / s (Markstein); outside
+// the range of s where neither over- nor underflows, by division.  (Checking d r for being
+// near to a half and dividing only then took a branch in two warps out of three, since a
+// bf16 x lies exactly half way in one case of 500: 254 us against 115.)  Adding and
+// subtracting 1.5 * 2^23 rounds to a whole number, ties to even; four codes are gathered as
+// one float, whose low 16 bits they are once 2^23 is added.
+__device__ __forceinline__ uint2 codes_of(const float* x, float s, float b) {
   constexpr float kRound = 12582912.f, kGather = 8388608.f - 128.f * 4369.f;      // 4369 = 1 + 16 + 256 + 4096
   if (!(s > 1e-30f && s < 1e36f)) {
     float y[16];
@@ -76,17 +100,20 @@ __device__ __forceinline__ uint2 codes_of(const float (&x)[16], float s, float b
     return codes_by_division(y, s, b);
   }
   const float r = __frcp_rn(s);
+  const F2 r2 = pair2(r, r), ns = pair2(-s, -s), nb = pair2(-b, -b);
+  const F2 up = pair2(kRound, kRound), down = pair2(-kRound, -kRound), k256 = pair2(256.f, 256.f);
+  auto codes2 = [&](float x0, float x1) {
+    const F2 d = add2(pair2(x0, x1), nb), q0 = mul2(d, r2);
+    float t0, t1;
+    halves(fma2(fma2(q0, ns, d), r2, q0), t0, t1);
+    return add2(add2(pair2(fminf(fmaxf(t0, 128.f), 143.f), fminf(fmaxf(t1, 128.f), 143.f)), up), down);
+  };
   uint32_t four[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    float sum = 0.f;
-#pragma unroll
-    for (int j = 3; j >= 0; --j) {
-      const float d = __fsub_rn(x[4 * q + j], b), q0 = __fmul_rn(d, r), t = fmaf(fmaf(-q0, s, d), r, q0);
-      const float c = (fminf(fmaxf(t, 128.f), 143.f) + kRound) - kRound;
-      sum = j == 3 ? c : fmaf(sum, 16.f, c);
-    }
-    four[q] = __float_as_uint(sum + kGather);
+    float even, odd;
+    halves(fma2(codes2(x[4 * q + 2], x[4 * q + 3]), k256, codes2(x[4 * q], x[4 * q + 1])), even, odd);
+    four[q] = __float_as_uint(fmaf(odd, 16.f, even) + kGather);
   }
   return make_uint2(low2(four[0], four[1]), low2(four[2], four[3]));
 }
@@ -100,18 +127,36 @@ __device__ __forceinline__ float fifteenth(float x) {
   return fmaf(fmaf(-15.f, q, x), c, q);
 }
 
-// 16 channels a thread, 2 threads a group of 32, ROWS rows a thread.  Rows go in the order
-// (token, head) in which the projections leave them, so the reads are contiguous.  Bound by
-// the arithmetic of the codes: 3.4 TB/s for 4 x 8191 tokens of 16 heads of 128 (104 us; its
-// reads and writes alone would take 54), with every issue slot in three used.
+// the range of 16 channels held as pairs (a NaN among them gives NaN)
+template <typename T> struct TwoOf;
+template <> struct TwoOf<__half> { using type = __half2; };
+template <> struct TwoOf<__nv_bfloat16> { using type = __nv_bfloat162; };
+template <typename T> using Two = typename TwoOf<T>::type;
+template <int N, typename P>
+__device__ __forceinline__ void two_range(const P* w, float& lo, float& hi) {
+  P a = w[0], b = w[0];
+#pragma unroll
+  for (int j = 1; j < N; ++j) {
+    a = __hmin2_nan(a, w[j]);
+    b = __hmax2_nan(b, w[j]);
+  }
+  lo = min_nan(to_f(a.x), to_f(a.y));
+  hi = max_nan(to_f(b.x), to_f(b.y));
+}
+
+// A group of 32 channels a thread, ROWS rows a thread.  Rows go in the order (token, head) in
+// which the projections leave them, so the reads are contiguous.  Bound by the arithmetic of
+// the codes, some 14 operations a channel: 4.5 TB/s for 4 x 8191 tokens of 16 heads of 128
+// (78 us; its reads and writes alone would take 54).  With 16 channels a thread, what a row
+// costs once was paid twice: 91 us, though a call of a few tokens took 2.1 us instead of 2.3.
 template <typename T, bool VEC, int ROWS>
-__global__ void __launch_bounds__(256) kv4_append_k(const Kv4AppendArgs a) {
+__global__ void __launch_bounds__(256, ROWS == 1 ? 4 : sizeof(T) == 4 ? 2 : 3) kv4_append_k(const Kv4AppendArgs a) {
   const int which = blockIdx.y;                       // 0: keys, 1: values
-  const int D = which ? a.Dv : a.D, per = D / 16, rows = 256 / per;
+  const int D = which ? a.Dv : a.D, per = D / kGroup, rows = 256 / per;
   const int ty = threadIdx.x / per, part = threadIdx.x - ty * per;
   const unsigned seq = blockIdx.x / a.blocks, block = blockIdx.x - seq * a.blocks;
   const long long b = seq;
-  const T* x = static_cast<const T*>(which ? a.v : a.k) + b * (which ? a.sv_b : a.sk_b) + 16 * part;
+  const T* x = static_cast<const T*>(which ? a.v : a.k) + b * (which ? a.sv_b : a.sk_b) + kGroup * part;
   const long long sh = which ? a.sv_h : a.sk_h, sl = which ? a.sv_l : a.sk_l;
   const unsigned total = static_cast<unsigned>(a.L) * a.Hk, Hk = a.Hk;
   const unsigned long long begin = static_cast<unsigned long long>(block) * (rows * ROWS);
@@ -135,42 +180,40 @@ __global__ void __launch_bounds__(256) kv4_append_k(const Kv4AppendArgs a) {
     }
   }
   constexpr int N = 16 / sizeof(T);                   // elements a 16-byte load
-  uint4 raw[VEC ? ROWS : 1][16 / N];
+  uint4 raw[VEC ? ROWS : 1][kGroup / N];
   if (VEC) {
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
       if (!idle && r0 + i * rows < total) {
 #pragma unroll
-        for (int j = 0; j < 16 / N; ++j) raw[i][j] = *reinterpret_cast<const uint4*>(x + hs[i] * sh + ls[i] * sl + j * N);
+        for (int j = 0; j < kGroup / N; ++j) raw[i][j] = *reinterpret_cast<const uint4*>(x + hs[i] * sh + ls[i] * sl + j * N);
       }
     }
   }
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
+    if (idle || r0 + i * rows >= total) break;
     const unsigned l = ls[i], h = hs[i];
-    const bool live = !idle && r0 + i * rows < total;         // pairs of threads are live or not together
-    float v[16];
+    float v[kGroup];
+    if (VEC) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = 0.f;
-    if (live) {
-      if (VEC) {
+      for (int j = 0; j < kGroup / N; ++j) {
+        const T* e = reinterpret_cast<const T*>(&raw[i][j]);
 #pragma unroll
-        for (int j = 0; j < 16 / N; ++j) {
-          const T* e = reinterpret_cast<const T*>(&raw[i][j]);
-#pragma unroll
-          for (int k = 0; k < N; ++k) v[j * N + k] = to_f(e[k]);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = to_f(x[h * sh + l * sl + j]);
+        for (int k = 0; k < N; ++k) v[j * N + k] = to_f(e[k]);
       }
-    }
-    float lo = v[0], hi = v[0];
+    } else {
 #pragma unroll
-    for (int j = 1; j < 16; ++j) { lo = min_nan(lo, v[j]); hi = max_nan(hi, v[j]); }
-    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, 1));
-    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, 1));
-    if (!live) continue;
+      for (int j = 0; j < kGroup; ++j) v[j] = to_f(x[h * sh + l * sl + j]);
+    }
+    float lo, hi;
+    if constexpr (VEC && sizeof(T) == 2) {
+      two_range<kGroup / 2>(reinterpret_cast<const Two<T>*>(raw[i]), lo, hi);
+    } else {
+      lo = hi = v[0];
+#pragma unroll
+      for (int j = 1; j < kGroup; ++j) { lo = min_nan(lo, v[j]); hi = max_nan(hi, v[j]); }
+    }
     const unsigned long long t = static_cast<unsigned long long>(start) + l;
     if (t >= static_cast<unsigned long long>(a.cap)) {        // a start given on the device that leaves the cache
       record_error(a.err, kErrBadArgument);
@@ -179,14 +222,12 @@ __global__ void __launch_bounds__(256) kv4_append_k(const Kv4AppendArgs a) {
     const __nv_bfloat16 s16 = __float2bfloat16_rn(fifteenth(__fsub_rn(hi, lo)));
     const float s = __bfloat162float(s16);
     const __nv_bfloat16 b16 = __float2bfloat16_rn(__fsub_rn(lo, __fmul_rn(128.f, s)));
-    const uint2 w = codes_of(v, s, __bfloat162float(b16));
+    const float b32 = __bfloat162float(b16);
     const long long out = (b * a.Hk + h) * a.cap + static_cast<long long>(t);
-    reinterpret_cast<uint2*>(which ? a.v_codes : a.k_codes)[out * per + part] = w;
-    if ((part & 1) == 0) {
-      const __nv_bfloat162 pr = __halves2bfloat162(s16, b16);
-      reinterpret_cast<uint32_t*>(which ? a.v_params : a.k_params)[out * (D / kGroup) + part / 2] =
-          *reinterpret_cast<const uint32_t*>(&pr);
-    }
+    const uint2 w = codes_of(v, s, b32), u = codes_of(v + 16, s, b32);
+    reinterpret_cast<uint4*>(which ? a.v_codes : a.k_codes)[out * per + part] = make_uint4(w.x, w.y, u.x, u.y);
+    const __nv_bfloat162 pr = __halves2bfloat162(s16, b16);
+    reinterpret_cast<uint32_t*>(which ? a.v_params : a.k_params)[out * per + part] = *reinterpret_cast<const uint32_t*>(&pr);
   }
 }
 
@@ -906,12 +947,13 @@ int attn_launch(const Kv4AttnArgs& a, cudaStream_t st) {
 int kv4_append(Kv4AppendArgs a, int type, cudaStream_t st) {
   if (a.D % kGroup || a.Dv % kGroup || a.D < kGroup || a.Dv < kGroup || a.D > 4096 || a.Dv > 4096) return 1;
   if (a.B * a.L * a.Hk == 0) return 0;
-  const int widest = a.D > a.Dv ? a.D : a.Dv, rows = 256 / (widest / 16);     // rows a block takes at once
   if (a.L * a.Hk > 0x7fffffffLL - 65536) return 2;
-  // four rows a thread, whose loads overlap, once that still makes several blocks an SM; one row below (300 tokens
-  // of 16 heads of 64: 2.6 us against 4.1)
-  const int each = a.B * ((a.L * a.Hk + 4 * rows - 1) / (4 * rows)) >= 148 * 4 ? 4 : 1;
-  a.blocks = static_cast<unsigned>((a.L * a.Hk + each * rows - 1) / (each * rows));
+  const int widest = a.D > a.Dv ? a.D : a.Dv;
+  // two rows a thread, whose loads overlap, once that still makes 16 blocks an SM (4 x 8191 tokens of 16 heads of 128:
+  // 78 us against 84); one row below (2 x 4096 tokens of 16 heads of 64: 11 us against 16)
+  const int each = a.B * a.L * a.Hk * (widest / kGroup) >= 2LL * 256 * 148 * 16 ? 2 : 1;
+  const int rows = each * (256 / (widest / kGroup));       // rows a block takes
+  a.blocks = static_cast<unsigned>((a.L * a.Hk + rows - 1) / rows);
   if (a.B * a.blocks > 0x7fffffffLL) return 2;
   const dim3 grid(static_cast<unsigned>(a.B * a.blocks), 2);
   const int es = type == 0 ? 4 : 2;
@@ -920,9 +962,9 @@ int kv4_append(Kv4AppendArgs a, int type, cudaStream_t st) {
   };
   const bool vec = al(a.k, a.sk_b, a.sk_h, a.sk_l) && al(a.v, a.sv_b, a.sv_h, a.sv_l);
 #define VAGUS_KV4_APPEND(T)                                              \
-  if (vec && each == 4) kv4_append_k<T, true, 4><<<grid, 256, 0, st>>>(a); \
+  if (vec && each == 2) kv4_append_k<T, true, 2><<<grid, 256, 0, st>>>(a); \
   else if (vec) kv4_append_k<T, true, 1><<<grid, 256, 0, st>>>(a);        \
-  else if (each == 4) kv4_append_k<T, false, 4><<<grid, 256, 0, st>>>(a); \
+  else if (each == 2) kv4_append_k<T, false, 2><<<grid, 256, 0, st>>>(a); \
   else kv4_append_k<T, false, 1><<<grid, 256, 0, st>>>(a)
   if (type == 0) { VAGUS_KV4_APPEND(float); }
   else if (type == 1) { VAGUS_KV4_APPEND(__half); }
