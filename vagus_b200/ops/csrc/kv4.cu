@@ -59,30 +59,6 @@ __device__ __noinline__ uint2 codes_by_division(const float* x, float s, float b
   return make_uint2(w[0], w[1]);
 }
 
-// Two floats an operation.
-using F2 = unsigned long long;
-__device__ __forceinline__ F2 pair2(float a, float b) {
-  F2 d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
-  return d;
-}
-__device__ __forceinline__ void halves(F2 x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
-__device__ __forceinline__ F2 add2(F2 a, F2 b) {
-  F2 d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  F2 d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  F2 d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-
 // The same in operations on two channels at once where there is one (the scalar ones made
 // the append 107 us instead of 91).  q0 = d r with the correctly rounded reciprocal r of s,
 // corrected once by its exact remainder, is the correctly rounded d / s (Markstein); outside

@@ -36,6 +36,20 @@ struct alignas(16) Vec {
   T v[N];
 };
 
+// two values, neighbours in a vector
+__device__ __forceinline__ void put2(float* d, float a, float b) { d[0] = a; d[1] = b; }
+__device__ __forceinline__ void put2(__half* d, float a, float b) { *reinterpret_cast<__half2*>(d) = __floats2half2_rn(a, b); }
+__device__ __forceinline__ void put2(__nv_bfloat16* d, float a, float b) {
+  *reinterpret_cast<__nv_bfloat162*>(d) = __floats2bfloat162_rn(a, b);
+}
+
+// two channel pairs by their angles, w = (cos, cos, sin, sin)
+__device__ __forceinline__ void turn2(F2& xa, F2& xb, float4 w) {
+  const F2 c = pair2(w.x, w.y), s = pair2(w.z, w.w), a = xa;
+  xa = fma2(a, c, mul2(xb, pair2(-w.z, -w.w)));
+  xb = fma2(a, s, mul2(xb, c));
+}
+
 constexpr int kThreads = 256;
 constexpr int kMaxAngles = 4096;     // pairs of angles of a CTA's tokens in shared memory
 
@@ -66,6 +80,8 @@ __device__ __forceinline__ void row_of(const RotaryArgs& a, long long b, long lo
   }
 }
 
+constexpr int ctas_per_sm(bool inter, int size) { return inter ? 8 : size == 4 ? 6 : 5; }
+
 // blockDim = (items of a head, rows); the rows are `across` heads of one token or, where the
 // heads are few, of several; an item is one 16-byte vector, or for the half
 // layout's rotated channels the two vectors that pair up.  The angles of an item's P pairs
@@ -73,10 +89,11 @@ __device__ __forceinline__ void row_of(const RotaryArgs& a, long long b, long lo
 // threads read neighbouring 16 bytes (item-major, 8 threads met in 2 of 8 bank groups).
 // A head's address is worked out once and its tokens follow.  Many resident threads matter
 // more than loads held ahead in registers (rows' loads taken two to four at a time: 146 to
-// 187 us for both directions of 4 x 4096 tokens of 32 heads of 128 in bf16, 105 so: 5.0
-// TB/s, and 6.2 TB/s in fp32, which has half the arithmetic a byte).
+// 187 us for both directions of 4 x 4096 tokens of 32 heads of 128 in bf16), and in 16 bits
+// so does the arithmetic a byte: two pairs an operation take 93 us where one takes 105 (5.6
+// TB/s; fp32 6.3 TB/s).
 template <typename T, bool INTER>
-__global__ void __launch_bounds__(kThreads, INTER ? 8 : 6) rotary_vec_k(const RotaryArgs a, int tokens, int across) {
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(INTER, sizeof(T))) rotary_vec_k(const RotaryArgs a, int tokens, int across) {
   constexpr int N = Vec<T>::N, P = INTER ? N / 2 : N;
   extern __shared__ __align__(16) float2 cs[];                    // [tokens][R / 2]
   __shared__ long long q_at[kThreads], k_at[kThreads];            // where a token's heads begin
@@ -87,8 +104,10 @@ __global__ void __launch_bounds__(kThreads, INTER ? 8 : 6) rotary_vec_k(const Ro
     const int k = i / half, p = i - k * half;
     const unsigned t = t0 + k, b = t / L, l = t - b * L;
     const int it = p / P, e = p - it * P;
-    cs[k * half + (e / 2 * (half / P) + it) * 2 + e % 2] =
-        angle_of(static_cast<double>(position_of(a, b, l)), a.inv[p], a.scale, a.sign);
+    const float2 w = angle_of(static_cast<double>(position_of(a, b, l)), a.inv[p], a.scale, a.sign);
+    float* to = reinterpret_cast<float*>(cs + k * half + (e / 2 * (half / P) + it) * 2) + e % 2;
+    to[0] = w.x;
+    to[2] = w.y;
     if (p == 0) {
       q_at[k] = b * a.sq_b + l * a.sq_l;
       k_at[k] = b * a.sk_b + l * a.sk_l;
@@ -116,28 +135,26 @@ __global__ void __launch_bounds__(kThreads, INTER ? 8 : 6) rotary_vec_k(const Ro
         if (item < rot) {
 #pragma unroll
           for (int e = 0; e < N; e += 4) {
-            const float4 w = c[e / 4 * rot];
-            float xa = to_f(x.v[e]), xb = to_f(x.v[e + 1]);
-            x.v[e] = from_f<T>(xa * w.x - xb * w.y);
-            x.v[e + 1] = from_f<T>(xa * w.y + xb * w.x);
-            xa = to_f(x.v[e + 2]);
-            xb = to_f(x.v[e + 3]);
-            x.v[e + 2] = from_f<T>(xa * w.z - xb * w.w);
-            x.v[e + 3] = from_f<T>(xa * w.w + xb * w.z);
+            F2 xa = pair2(to_f(x.v[e]), to_f(x.v[e + 2])), xb = pair2(to_f(x.v[e + 1]), to_f(x.v[e + 3]));
+            turn2(xa, xb, c[e / 4 * rot]);
+            float a0, a1, b0, b1;
+            halves(xa, a0, a1);
+            halves(xb, b0, b1);
+            put2(x.v + e, a0, b0);
+            put2(x.v + e + 2, a1, b1);
           }
         }
       } else if (pair) {
         Vec<T> y = *reinterpret_cast<const Vec<T>*>(src + half);
 #pragma unroll
         for (int e = 0; e < N; e += 2) {
-          const float4 w = c[e / 2 * rot];
-          float xa = to_f(x.v[e]), xb = to_f(y.v[e]);
-          x.v[e] = from_f<T>(xa * w.x - xb * w.y);
-          y.v[e] = from_f<T>(xa * w.y + xb * w.x);
-          xa = to_f(x.v[e + 1]);
-          xb = to_f(y.v[e + 1]);
-          x.v[e + 1] = from_f<T>(xa * w.z - xb * w.w);
-          y.v[e + 1] = from_f<T>(xa * w.w + xb * w.z);
+          F2 xa = pair2(to_f(x.v[e]), to_f(x.v[e + 1])), xb = pair2(to_f(y.v[e]), to_f(y.v[e + 1]));
+          turn2(xa, xb, c[e / 2 * rot]);
+          float a0, a1, b0, b1;
+          halves(xa, a0, a1);
+          halves(xb, b0, b1);
+          put2(x.v + e, a0, a1);
+          put2(y.v + e, b0, b1);
         }
         *reinterpret_cast<Vec<T>*>(dst + half) = y;
       }
@@ -182,11 +199,14 @@ template <typename T>
 int launch(const RotaryArgs& a, cudaStream_t st) {
   constexpr int N = Vec<T>::N;
   const int half = a.R / 2;
-  // tokens a CTA: as many as its threads have angles for at once, fewer while that leaves the GPU no two full waves
-  // (4610 tokens of 40 heads of 128, 64 channels rotated, bf16: 18.9 us interleaved and 22.2 us half at 12 CTAs an SM,
-  // 22.2 and 22.8 us at 4)
-  int tokens = half >= kThreads ? 1 : kThreads / half;
-  while (tokens > 1 && (a.B * a.L + tokens - 1) / tokens < 148 * 12) --tokens;
+  // tokens a CTA: up to as many as its threads have angles for at once, the share whose waves over the GPU end first
+  // (a CTA's start counts for two tokens).  4610 tokens of 40 heads of 128, 64 channels rotated, bf16: half 7 a CTA 19.4
+  // us, 2 a CTA 22.7; interleaved 4 a CTA 16.1, 2 a CTA 17.1
+  const long long slots = 148LL * ctas_per_sm(a.interleaved, sizeof(T));
+  auto length = [&](int t) { return ((a.B * a.L + t - 1) / t + slots - 1) / slots * (t + 2); };
+  int tokens = half >= kThreads ? 1 : half <= 8 ? 32 : kThreads / half;
+  for (int t = tokens - 1; t > 0; --t)
+    if (length(t) < length(tokens)) tokens = t;
   while (tokens > 1 && static_cast<long long>(tokens) * (a.H + a.Hk) * a.D > 1 << 30) --tokens;
   const long long grid = (a.B * a.L + tokens - 1) / tokens;
   if (a.B * a.L > 0x7fff0000LL) return 2;                // tokens are counted in 32 bits, and so is what one of them holds
