@@ -12,6 +12,7 @@ angles negated.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from ._core import native
 
@@ -45,14 +46,28 @@ def rotary_ref(x, positions, inv_freq, layout: str = "interleaved", scale: float
 
 class _Rotary(torch.autograd.Function):
     """q and, unless it is None, k.  The backward applies this function with the
-    angles negated, so it is differentiable itself."""
+    angles negated and a tangent is rotated like its primal, so derivatives of
+    either mode can be taken again."""
 
     @staticmethod
     def forward(ctx, q, k, pos, offset, inv, interleaved, scale, sign):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(pos, inv)
+        ctx.save_for_forward(pos, inv)
         ctx.meta = (offset, interleaved, scale, sign)
+        ctx.shapes = (q.shape, None if k is None else k.shape)
         return native().rotary(q, k, pos, offset, inv, interleaved, scale, sign)
+
+    @staticmethod
+    def jvp(ctx, tq, tk, tpos, toffset, tinv, *_):
+        if tinv is not None:
+            raise NotImplementedError("rotary: no derivative with respect to inv_freq on the GPU")
+        pos, inv = ctx.saved_tensors
+        offset, interleaved, scale, sign = ctx.meta
+        of_q, of_k = ctx.shapes
+        tq = tk.new_zeros(of_q) if tq is None else tq
+        tk = tq.new_zeros(of_k) if tk is None and of_k is not None else tk
+        return _run(tq, tk, pos, offset, inv, interleaved, scale, sign)
 
     @staticmethod
     def backward(ctx, dq, dk):
@@ -60,12 +75,20 @@ class _Rotary(torch.autograd.Function):
         offset, interleaved, scale, sign = ctx.meta
         if dq is None and dk is None:
             return (None,) * 8
-        run = _Rotary.apply if torch.is_grad_enabled() else native().rotary
         if dq is None:
-            gk, gq = run(dk, None, pos, offset, inv, interleaved, scale, -sign)
+            gk, gq = _run(dk, None, pos, offset, inv, interleaved, scale, -sign)
         else:
-            gq, gk = run(dq, dk, pos, offset, inv, interleaved, scale, -sign)
+            gq, gk = _run(dq, dk, pos, offset, inv, interleaved, scale, -sign)
         return gq, gk, None, None, None, None, None, None
+
+
+def _run(q, k, *args):
+    """The kernel, through the function above where a derivative of either mode may be
+    taken (inside a dual level any tensor may carry a tangent)."""
+    if (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))) \
+            or forward_ad._current_level >= 0:
+        return _Rotary.apply(q, k, *args)
+    return native().rotary(q, k, *args)
 
 
 def _check(q, k, positions, inv_freq):
@@ -90,7 +113,8 @@ def rotary(q, k, positions, inv_freq, layout: str = "interleaved", scale: float 
 
     ``positions``: an int (token l sits at positions + l), or an int32 / int64
     tensor (L,) or (B, L).  ``inv_freq``: (R/2,) angle per step of position,
-    float64 (other float types are converted), R <= D.  Gradients flow to q and k."""
+    float64 (other float types are converted), R <= D.  Derivatives of both modes
+    are taken with respect to q and k."""
     if layout not in LAYOUTS:
         raise ValueError(f"rotary layout must be one of {LAYOUTS}, got {layout!r}")
     if isinstance(positions, int):
@@ -104,8 +128,5 @@ def rotary(q, k, positions, inv_freq, layout: str = "interleaved", scale: float 
         y = rotary_ref(q, positions, inv_freq, layout, scale)
         return y if k is None else (y, rotary_ref(k, positions, inv_freq, layout, scale))
     # on the GPU the binding checks the arguments (the same conditions)
-    run = native().rotary
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        run = _Rotary.apply
-    out = run(q, k, pos, offset, inv_freq, layout == "interleaved", scale, 1.0)
+    out = _run(q, k, pos, offset, inv_freq, layout == "interleaved", scale, 1.0)
     return out[0] if k is None else out
