@@ -1,12 +1,14 @@
 """The long-context streaming kernels at calls that the documentation allows and that
-lie off the common path: forward-mode derivatives of the rotation."""
+lie off the common path: forward-mode derivatives of the rotation, very many short
+prompts."""
 
 import pytest
 import torch
 import torch.autograd.forward_ad as fwad
 
 from vagus_b200 import ops
-from tests.test_stream_ops import LAYOUTS, frequencies
+from tests.test_stream_ops import LAYOUTS, attention_64, frequencies
+from tests.test_stream_ops_gpu import filled
 
 pytestmark = pytest.mark.gpu
 
@@ -78,3 +80,24 @@ def test_rotary_reverse_over_forward():
     probe = q.clone().requires_grad_()
     (want,) = torch.autograd.grad(ops.rotary(probe, None, 7, inv), probe, w)
     assert torch.equal(got, want)
+
+
+# --------------------------------------------------------------------- attention --
+
+@pytest.mark.parametrize("B,H", [(4095, 16), (4097, 16)])
+def test_attention_of_more_heads_than_a_grid_dimension(B, H):
+    """Batch times heads on both sides of 65535, with blocks of queries long enough to be served from unpacked values."""
+    Lq = n = 128
+    c = filled(B, 1, n, 64, 64)
+    q = torch.randn(B, Lq, H, 64, device=DEV).bfloat16().transpose(1, 2)
+    got = ops.int4_attention(q, c, n)
+    assert got.shape == (B, H, Lq, 64)
+    k, v = ops.int4_read(c, 0, n)
+    # the output and each probability round to bf16 (2^-8 each); served from unpacked values, an exponential is a fit
+    # good to 7.5e-5, numerator and sum, and a hidden token weighs up to 2^-126 instead of nothing; a score is an fp32
+    # sum of 64 products, off by at most 64 * 2^-24 of their sizes' sum over 8, numerator and sum
+    slack = 2 ** -8 + 2e-4 + 2 * 64 * 2 ** -24 * 64 * float(q.abs().max()) * float(k.abs().max()) / 8
+    tail = n * 2.0 ** -126 * float(v.abs().max())
+    for b in (0, 2048, B - 1):
+        want, mag = attention_64(q[b:b + 1], k[b:b + 1], v[b:b + 1], [n], True)
+        assert ((got[b:b + 1].double() - want).abs() <= 2 ** -8 * want.abs() + slack * mag + tail).all()

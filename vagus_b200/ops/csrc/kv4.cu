@@ -1000,6 +1000,7 @@ int kv4_attn_plan(Kv4AttnArgs& a, long long most_tokens) {
 // tokens of 16 heads of 64: 103 / 377 / 741 against 381 / 383 / 385.
 bool kv4_attn_unpack_first(const Kv4AttnArgs& a) {
   if (a.lengths || a.Lq < 128 || a.length < 128 || a.Lq > a.length || a.D != a.Dv || a.B * a.H == 0) return false;
+  if (a.B * a.H > 65535) return false;       // that attention's grid holds batch times heads in its second dimension
   const double tiles = (static_cast<double>(a.H / a.Hk) * a.Lq + 15) / 16, units = (a.length + kUnit - 1) / kUnit;
   const double here = 0.0052 * a.B * a.Hk * tiles * units;
   const long long ctas = a.B * a.H * ((a.Lq + 127) / 128), wave = a.D == 64 ? 296 : 148;
