@@ -43,11 +43,21 @@ def check_error() -> None:
 class _Bf16Cache:
     """bf16 compute copies of fp32 master weights, rebuilt when the master
     changes (its autograd version counter moves on every in-place update).  An
-    entry holds a weak reference to its master: a new tensor that takes a dead
-    one's id and memory is another master."""
+    entry holds weak references to its masters: a new tensor that takes a dead
+    one's id and memory is another master, and a dead one's entries are dropped."""
 
     def __init__(self):
         self._d: dict = {}
+
+    def _refs(self, key, ws):
+        """Weak references to an entry's masters; the first of them to die takes the entry with it."""
+        entries = self._d
+
+        def drop(ref):
+            hit = entries.get(key)
+            if hit is not None and any(r is ref for r in hit[3]):       # not a newer entry of the same ids
+                entries.pop(key, None)
+        return [weakref.ref(w, drop) for w in ws]
 
     def get(self, w: torch.Tensor) -> torch.Tensor:
         if w.dtype == torch.bfloat16:
@@ -55,10 +65,10 @@ class _Bf16Cache:
         key = id(w)
         ver = w._version
         hit = self._d.get(key)
-        if hit is not None and hit[0] == ver and hit[1] == w.data_ptr() and hit[3]() is w:
+        if hit is not None and hit[0] == ver and hit[1] == w.data_ptr() and hit[3][0]() is w:
             return hit[2]
         c = w.detach().to(torch.bfloat16).contiguous()
-        self._d[key] = (ver, w.data_ptr(), c, weakref.ref(w))
+        self._d[key] = (ver, w.data_ptr(), c, self._refs(key, [w]))
         return c
 
     def get_cat(self, ws: list[torch.Tensor]) -> torch.Tensor:
@@ -73,7 +83,7 @@ class _Bf16Cache:
         if hit is not None and hit[0] == vers and all(r() is w for r, w in zip(hit[3], ws)):
             return hit[2]
         c = torch.cat([w.detach().to(torch.bfloat16) for w in ws], 0).contiguous()
-        self._d[key] = (vers, None, c, [weakref.ref(w) for w in ws])
+        self._d[key] = (vers, None, c, self._refs(key, ws))
         return c
 
     def clear(self):
