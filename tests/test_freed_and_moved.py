@@ -1,10 +1,14 @@
 """What is kept beside a model's tensors goes with them: the bf16 compute copies of its
-weights are freed with the weights."""
+weights are freed with the weights, the 4-bit KV caches of open streams move with the
+model."""
 
 import gc
 
+import pytest
 import torch
 
+from vagus_b200 import ops
+from vagus_b200.models import build_model
 from vagus_b200.ops._core import _Bf16Cache
 
 
@@ -63,3 +67,55 @@ def test_an_address_and_an_id_taken_over():
         w = torch.full((16, 16), float(i))
         assert (cache.get(w) == i).all() and len(cache._d) == 1
         del w
+
+
+# ------------------------------------------------------------------- 4-bit cache --
+
+def streaming(**kw):
+    """A model with a 4-bit cache that holds 9 tokens of two streams."""
+    torch.manual_seed(0)
+    m = build_model("TransformerPP", dict(vocab_size=300, dim=64, layer_count=2, head_dim=32, context_len=64,
+                                          ffn_hidden_dim=128, **kw)).eval()
+    m.set_cache_bits(4)
+    m.reset_cache(2, 40)
+    m.decode_step(torch.randint(0, 300, (2, 9)))
+    return m
+
+
+def caches(m):
+    return [t for b in m.blocks for t in b.att.kv4.tensors()]
+
+
+def test_open_streams_move_with_the_model():
+    m = streaming().to("meta")
+    assert all(t.device.type == "meta" for t in caches(m) + [b.att.k_cache for b in m.blocks])
+    m.to_empty(device="cpu")
+    assert all(t.device.type == "cpu" for t in caches(m))
+    ops.int4_read(m.blocks[0].att.kv4, 0, 9)
+
+
+@pytest.mark.parametrize("cast", [lambda m: m.double(), lambda m: m.to(torch.bfloat16), lambda m: m.half().float()])
+def test_a_cast_leaves_the_codes_alone(cast):
+    m = streaming()
+    before = [t.clone() for t in caches(m)]
+    cast(m)
+    for a, b in zip(caches(m), before):
+        assert a.dtype == b.dtype and torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.gpu
+def test_a_model_moves_between_two_decode_steps():
+    ids = torch.randint(0, 300, (2, 3))
+    here, moved = streaming(), streaming()
+    want = here.decode_step(ids)
+    before = [t.clone() for t in caches(moved)]
+    moved.to("cuda")
+    assert all(a.is_cuda and torch.equal(a.cpu().view(torch.uint8), b.view(torch.uint8))
+               for a, b in zip(caches(moved), before))
+    got = moved.decode_step(ids.cuda())
+    # the same codes; sums of at most 128 products in fp32, under 20 one after another: 20 * 128 * 2^-24 < 2e-4
+    assert (got.cpu() - want).abs().max() < 1e-3 * want.abs().max()
+    moved.to("cpu")
+    nxt = torch.randint(0, 300, (2, 1))
+    want = here.decode_step(nxt)
+    assert (moved.decode_step(nxt) - want).abs().max() < 1e-3 * want.abs().max()

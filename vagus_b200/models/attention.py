@@ -153,6 +153,13 @@ class SoftmaxAttention(nn.Module, Mixer):
                              f"{self.value_head_dim}")
         self.cache_bits = bits
 
+    def _apply(self, fn, recurse=True):
+        """A 4-bit cache moves with the buffers; its codes and parameters keep their types."""
+        super()._apply(fn, recurse)
+        if self.kv4 is not None:
+            self.kv4 = self.kv4.to(self.k_cache.device)
+        return self
+
     def reset_cache(self, batch_size: int, max_cache_len: int):
         device, dtype = infer_device(self), infer_dtype(self)
         Hk, Dh, Dvh = self.kv_head_count, self.head_dim, self.value_head_dim

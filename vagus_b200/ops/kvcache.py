@@ -76,6 +76,14 @@ class Int4KV:
     def tensors(self) -> tuple[torch.Tensor, ...]:
         return self.k_codes, self.k_params, self.v_codes, self.v_params
 
+    def to(self, device) -> "Int4KV":
+        """The cache on another device (itself, where it is there already).  From the
+        meta device, which holds nothing, a cache of unspecified content."""
+        device = torch.device(device)
+        if device == self.k_codes.device:
+            return self
+        return Int4KV(*(torch.empty_like(t, device=device) if t.is_meta else t.to(device) for t in self.tensors()))
+
     @property
     def batch(self) -> int:
         return self.k_codes.shape[0]
