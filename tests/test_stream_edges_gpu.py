@@ -1,6 +1,6 @@
 """The long-context streaming kernels at calls that the documentation allows and that
 lie off the common path: forward-mode derivatives of the rotation, very many short
-prompts."""
+prompts, writes that take two rows a thread."""
 
 import pytest
 import torch
@@ -101,3 +101,70 @@ def test_attention_of_more_heads_than_a_grid_dimension(B, H):
     for b in (0, 2048, B - 1):
         want, mag = attention_64(q[b:b + 1], k[b:b + 1], v[b:b + 1], [n], True)
         assert ((got[b:b + 1].double() - want).abs() <= 2 ** -8 * want.abs() + slack * mag + tail).all()
+
+
+# ------------------------------------------------------------------- 4-bit cache --
+
+def two_rows_a_thread(B, L, Hk, D, Dv):
+    """Whether a write is large enough for the form that takes two rows a thread."""
+    return B * L * Hk * (max(D, Dv) // 32) >= 2 * 256 * 148 * 16
+
+
+def equal_to_the_plain_form(c, k, v, start):
+    """Bit for bit, what was written and what was left alone (the plain form runs on the CPU)."""
+    want = ops.Int4KV.empty(c.batch, c.kv_heads, c.capacity, c.head_dim, c.value_dim)
+    ops.int4_append(want, k.cpu(), v.cpu(), start if isinstance(start, int) else start.cpu())
+    return all(torch.equal(a.cpu().view(torch.uint8), b.view(torch.uint8)) for a, b in zip(c.tensors(), want.tensors()))
+
+
+# rows of a block's threads: 256 / (D / 32) of the tensor at hand.  Heads that do not divide them, more heads than
+# there are of them, one head, idle threads (D = 96), unequal dims (the narrower tensor takes fewer blocks), odd lengths
+@pytest.mark.parametrize("B,L,Hk,D,Dv,dtype", [
+    (2, 30401, 5, 128, 128, torch.bfloat16), (1, 101111, 3, 64, 128, torch.float16), (1, 101111, 3, 128, 64, torch.float32),
+    (1, 1013, 300, 128, 128, torch.bfloat16), (2, 606209, 1, 32, 32, torch.bfloat16), (1, 134713, 3, 96, 96, torch.float16),
+    (3, 2311, 44, 32, 128, torch.float32)])
+def test_append_of_two_rows_a_thread(B, L, Hk, D, Dv, dtype):
+    assert two_rows_a_thread(B, L, Hk, D, Dv)
+    k = torch.randn(B, L, Hk, D, device=DEV).add_(0.5 * torch.randn(D, device=DEV)).to(dtype).transpose(1, 2)
+    v = torch.randn(B, Hk, L, Dv, device=DEV).to(dtype)
+    for start in (3, torch.randint(0, 20, (B,), device=DEV)):
+        c = ops.Int4KV.empty(B, Hk, L + 20, D, Dv, device=DEV)
+        ops.int4_append(c, k, v, start)
+        assert equal_to_the_plain_form(c, k, v, start)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_append_of_two_rows_a_thread_off_16_bytes(dtype):
+    B, L, Hk, D = 1, 101111, 3, 128
+    assert two_rows_a_thread(B, L, Hk, D, D)
+    packed = torch.randn(B, L, 2 * Hk * D + 1, device=DEV).to(dtype)[..., 1:]
+    k, v = (t.unflatten(-1, (Hk, D)).transpose(1, 2) for t in packed.chunk(2, -1))
+    c = ops.Int4KV.empty(B, Hk, L + 9, D, device=DEV)
+    ops.int4_append(c, k, v, 7)
+    assert equal_to_the_plain_form(c, k, v, 7)
+
+
+@pytest.mark.parametrize("Hk,L", [(5, 30401), (70, 2171)])
+def test_append_of_two_rows_a_thread_past_the_end(Hk, L):
+    """Sequences that start before the cache and reach past its end: tokens inside are written, and nothing else."""
+    B, D = 2, 128
+    assert two_rows_a_thread(B, L, Hk, D, D)
+    k, v = (torch.randn(B, Hk, L, D, device=DEV).bfloat16() for _ in range(2))
+    cap = (L + 15) // 16 * 16
+    c = ops.Int4KV.empty(B, Hk, cap, D, device=DEV)
+    for t in c.tensors():
+        t.fill_(1)
+    left, right = -37, cap - L + 41
+    ops.int4_append(c, k, v, torch.tensor([left, right], device=DEV))
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="outside"):
+        ops.check_error()
+    want = ops.Int4KV.empty(B, Hk, cap, D)
+    for t in want.tensors():
+        t.fill_(1)
+    for b, (at, first, last) in enumerate(((0, 37, L), (right, 0, L - 41))):
+        one = ops.Int4KV.empty(1, Hk, cap, D)
+        ops.int4_append(one, k[b:b + 1, :, first:last].cpu(), v[b:b + 1, :, first:last].cpu(), at)
+        for a, x in zip(want.tensors(), one.tensors()):
+            a[b, :, at:at + last - first] = x[0, :, at:at + last - first]
+    assert all(torch.equal(a.cpu().view(torch.uint8), b.view(torch.uint8)) for a, b in zip(c.tensors(), want.tensors()))
