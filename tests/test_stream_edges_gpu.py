@@ -1,13 +1,13 @@
 """The long-context streaming kernels at calls that the documentation allows and that
 lie off the common path: forward-mode derivatives of the rotation, very many short
-prompts, writes that take two rows a thread."""
+prompts, writes that take two rows a thread, and the same call made again."""
 
 import pytest
 import torch
 import torch.autograd.forward_ad as fwad
 
 from vagus_b200 import ops
-from tests.test_stream_ops import LAYOUTS, attention_64, frequencies
+from tests.test_stream_ops import LAYOUTS, attention_64, drafted, frequencies
 from tests.test_stream_ops_gpu import filled
 
 pytestmark = pytest.mark.gpu
@@ -168,3 +168,48 @@ def test_append_of_two_rows_a_thread_past_the_end(Hk, L):
         for a, x in zip(want.tensors(), one.tensors()):
             a[b, :, at:at + last - first] = x[0, :, at:at + last - first]
     assert all(torch.equal(a.cpu().view(torch.uint8), b.view(torch.uint8)) for a, b in zip(c.tensors(), want.tensors()))
+
+
+# ------------------------------------------------------------------------ replay --
+
+def replay(run):
+    """No sum in these kernels depends on the order of arrival: the same call gives the same bits."""
+    first = [t.clone() for t in run()]
+    busy = torch.randn(4096, 4096, device=DEV)
+    for i in range(4):
+        if i % 2:
+            busy @ busy                                # another load on the GPU ahead of it
+        for a, b in zip(run(), first):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B,H,Hk,Lq,T", [(32, 32, 8, 1, 8192), (2, 16, 8, 1, 40003), (8, 16, 16, 6, 4099), (1, 8, 8, 700, 4096),
+                                         (600, 4, 2, 1, 300)])
+def test_attention_replays(B, H, Hk, Lq, T, D):
+    c = filled(B, Hk, T, D, D)
+    q = torch.randn(B, H, Lq, D, device=DEV).bfloat16()
+    replay(lambda: [ops.int4_attention(q, c, T)])
+    lengths = torch.randint(0, T + 1, (B,), device=DEV)
+    replay(lambda: [ops.int4_attention(q, c, lengths)])
+
+
+def test_other_stream_kernels_replay():
+    k, v = torch.randn(2, 4, 5000, 128, device=DEV), torch.randn(2, 4, 5000, 64, device=DEV)
+    c = ops.Int4KV.empty(2, 4, 5008, 128, 64, device=DEV)
+    start = torch.tensor([3, 8], device=DEV)
+
+    def write():
+        ops.int4_append(c, k, v, start)
+        return [*c.tensors(), *ops.int4_read(c, start, 5000)]
+    replay(write)
+    q = torch.randn(2, 5000, 4, 128, device=DEV).bfloat16().requires_grad_()
+    g = torch.randn_like(q)
+    inv = frequencies(64).to(DEV)
+    for layout in LAYOUTS:
+        replay(lambda: [ops.rotary(q, None, 5, inv, layout=layout).detach(),
+                        torch.autograd.grad(ops.rotary(q, None, 5, inv, layout=layout), q, g)[0]])
+    for B, K, V in ((1, 4, 32000), (300, 3, 4099)):
+        target, draft, tokens, ua, us = drafted(B, K, V, device=DEV)
+        replay(lambda: ops.verify_draft(target, draft, tokens, ua, us))
+        replay(lambda: ops.verify_draft(target, None, tokens, ua, us))
