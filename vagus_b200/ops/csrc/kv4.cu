@@ -8,9 +8,12 @@
 // and not c: bf16 has 7 mantissa bits, so the bit pattern 0x4300 | c IS the
 // number 128 + c, and a pair of codes becomes a pair of values with one bitwise
 // operation and one bf16 fused multiply-add, exactly as the format defines them.
-// b is rounded to bf16 near -128 s, by at most 0.53 s; the codes are computed
-// from the rounded b, so this shifts the group's grid of 16 levels and adds no
-// error to a value inside it.
+// The codes are computed from the rounded b, so its rounding, e <= 2^-8 |min - 128 s|,
+// shifts the group's grid of 16 levels: a value inside the grid is off by s / 2 at most,
+// one at the group's edge by at most e + 0.06 s (the rounding of s over 15 of them), and
+// then the value itself rounds to bf16.  Groups near zero lose nothing by it (0.55 s at
+// worst in 40000 groups of unit variance), far ones do: 0.64 s at a mean of 5 times their
+// deviation, 0.93 s at 20, 1.7 s at 60, where a bf16 value's own rounding is 0.9 s.
 #include "common.cuh"
 #include "kernels.h"
 #include "mma.cuh"
@@ -322,14 +325,16 @@ __global__ void __launch_bounds__(256) kv4_read_few_k(const Kv4ReadArgs a) {
 //   whole; of the first and last item of its share it may have a part, which it leaves in
 //   slot 0 or 1 of its scratch, and a second kernel adds the parts of an item in order.
 //
-// What bounds it: the unpacking.  Of 16 tokens x 128 channels of K and V a warp does 64
-// shift / mask-or / fma triples, 16 products and 12 permutes, and the logic operations
-// issue at half rate next to fmas and products that share ports with them: 72 us for 2 x
-// 131067 tokens of 8 KV heads of 128 (4.7 TB/s), whose bytes alone take 52, and about the
-// same with its loads served by L2.  A ring of bulk copies into shared memory with 8, 12 or
-// 16 warps an SM, and scores formed one block ahead, all measured the same within 4 percent;
-// 4 or 5 CTAs an SM at head dim 64 too.  Loads two tiles ahead into registers are the
-// simplest of them.
+// What bounds it: latency.  Of 16 tokens x 128 channels of K and V a warp does 64 shift /
+// mask-or / fma triples, 16 products and 12 permutes in one chain from scores to products,
+// at 11 warps an SM; in the ragged batch of 32 single tokens over up to 8192 tokens the ALU
+// pipe (where the logic operations issue at half rate), DRAM and the issue slots are each
+// half busy, and the waits are fixed latencies and loads about equally.  2 x 131067 tokens
+// of 8 KV heads of 128 take 72 us (4.7 TB/s; their bytes alone 52), and about the same with
+// the loads served by L2.  A ring of bulk copies into shared memory with 8, 12 or 16 warps
+// an SM, and scores formed one block ahead, all measured the same within 4 percent; 4 or 5
+// CTAs an SM at head dim 64 too.  Loads two tiles ahead into registers are the simplest of
+// them.
 
 constexpr int kAttnWarps = 4;
 constexpr int kUnit = 32 * kAttnWarps;      // tokens
@@ -994,10 +999,13 @@ int kv4_attn_plan(Kv4AttnArgs& a, long long most_tokens) {
 }
 
 // Whether many query rows over equal lengths are better served by unpacking the values once and running the
-// tcgen05 attention on them.  The kernels above take 5.2 ns a unit and tile of 16 rows, on the whole GPU; the
-// other way takes the read, some 12 us of launches and, a wave of 128-row CTAs, 1.5 us per 128 tokens.  Measured, 16
-// heads of 128 over 8192 tokens: 55 / 177 / 341 us against 109 / 109 / 111 at 128 / 512 / 1024 rows; over 32768
-// tokens of 16 heads of 64: 103 / 377 / 741 against 381 / 383 / 385.
+// tcgen05 attention on them.  At head dim 128 the kernels above take 5.2 ns a unit and tile of 16 rows, on the whole
+// GPU; the other way takes the read, some 12 us of launches and, a wave of 128-row CTAs, 1.5 us per 128 tokens.
+// Measured, codes against unpacked.  16 heads of 128 over 8192 tokens: 62 / 103 / 124 / 146 / 187 / 351 us against 114
+// to 118 at 128 / 256 / 320 / 384 / 512 / 1024 rows; the rule changes sides between 320 and 384.  16 heads of 64 over
+// 32768 tokens: 122 / 218 / 269 / 306 / 361 / 396 / 765 against 386 to 392 at 128 / 256 / 320 / 384 / 448 / 512 / 1024.
+// There a tile takes about 2.9 ns, which the one constant does not know: the rule changes sides between 256 and 320
+// rows, and from there to 512 it takes the slower way.
 bool kv4_attn_unpack_first(const Kv4AttnArgs& a) {
   if (a.lengths || a.Lq < 128 || a.length < 128 || a.Lq > a.length || a.D != a.Dv || a.B * a.H == 0) return false;
   if (a.B * a.H > 65535) return false;       // that attention's grid holds batch times heads in its second dimension

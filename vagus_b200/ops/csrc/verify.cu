@@ -8,7 +8,10 @@
 //
 // The sums are held in 64 bits: with 10^5 candidates the 32-bit rounding of a
 // running sum moves a border past u once in a few hundred draws, and the token
-// would depend on the order of summation.
+// would depend on the order of summation.  That order follows from the batch, the
+// vocabulary and the alignment (they set the pieces and the width of the loads), so a
+// call repeats itself; a row alone and the same row in a batch may differ where u lies
+// within those sums' rounding of a border.
 //
 // What bounds it is one row of p and of q a request, or latency for few
 // requests: two dependent reads (the drafted tokens, their probabilities) before

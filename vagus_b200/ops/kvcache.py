@@ -8,9 +8,12 @@ step s and an offset b in bf16:
     c = clamp(round((x - b) / s) - 128, 0, 15),  and c stands for bf16((128 + c) s + b)
 
 (round: to nearest, ties to even; the steps in fp32).  That is 0.625 bytes a
-value against 2 of a bf16 cache, and a value is off by little more than half a
-step.  A group of equal values is held exactly (s = 0); a group that holds a NaN
-or an infinity stands for NaN; magnitudes up to 1e37 are representable.
+value against 2 of a bf16 cache.  A value is off by at most
+max(s / 2, 2^-8 |min - 128 s| + 0.06 s) and its own rounding to bf16: little more
+than half a step in groups near zero, more in groups whose minimum lies far from
+it (the rounding of b moves the grid, and values at the group's edge are clamped).
+A group of equal values is held to bf16 (s = 0); a group that holds a NaN or an
+infinity stands for NaN; magnitudes up to 1e37 are representable.
 
 ``int4_attention`` is attention over the values that the codes stand for, which
 ``int4_read`` returns: however a stream is cut into calls, a token sees the same
@@ -240,10 +243,17 @@ def int4_attention(q, cache: Int4KV, lengths, causal: bool = True):
     ``causal`` the queries are the last Lq of those tokens: query i sees the
     first lengths - Lq + i + 1 of them.  A query that sees nothing gives zeros.
     What the cache holds past a sequence's length has no effect; a NaN inside it
-    may reach every query of the call.  Inference only: no gradient flows.  The
-    kernels take bf16 queries and head dims 64 and 128, the plain form serves the
-    others; with many queries over equal lengths (an int) the values are unpacked
-    into a temporary bf16 copy first."""
+    may reach every query of the call.  Inference only: no derivative of either
+    mode flows.
+
+    The kernels take bf16 queries and head dims 64 and 128.  Scores, softmax sums and
+    accumulators are fp32; probabilities are rounded to bf16 for the product with the
+    values (2^-8 relative at most, unbiased), as in ``ops.attention``.  With many
+    queries over equal lengths (an int) the values are unpacked into a temporary bf16
+    copy first.  Other types and head dims take the plain form in fp32, which forms
+    all scores (and with lengths per sequence unpacks the whole capacity).  Refused with
+    a RuntimeError: batch x KV heads x tiles of 16 query rows x blocks of 128 tokens
+    (of the capacity, with lengths per sequence) of about 2^30 or more."""
     per, at = _place(lengths, "int4_attention: lengths")
     if cache.k_codes.is_cuda:
         o = native().kv4_attn(q, cache.k_codes, cache.k_params, cache.v_codes, cache.v_params, per, at, causal)

@@ -79,7 +79,9 @@ def verify_draft(target, draft, tokens, u_accept, u_sample, lengths=None):
     Returns ``(out, accepted)``: accepted (B,) int64, and out (B, K + 1) int64
     holding the accepted drafts, the token that follows, then -1.  A drafted
     token outside the vocabulary is rejected.  The next token is the first v
-    whose running sum of weights exceeds u_sample times their sum, in 64 bits;
+    whose running sum of weights exceeds u_sample times their sum, in 64 bits (the
+    order of the sums is fixed for given B, V, dtype and alignment; another could give a
+    neighbouring token only where u_sample lies within their rounding of a border);
     where nothing is left of max(p - q, 0) it is drawn from p, and a row without
     any weight gives token 0.  K = 0 draws one token from ``target``."""
     if target.is_cuda:                       # the binding checks the arguments by the same conditions
